@@ -31,12 +31,18 @@ NVCC_FLAGS = [
     "-Xptxas", "-v" if os.environ.get("H3_PTXAS_VERBOSE") else "-O3",
 ]
 
+# The C++ runtime must be the process's shared one (torch's): a linker whose
+# default is the static libstdc++ gives the module a second runtime, and an
+# error message that prints a number then crashes instead of raising.
+LINK_FLAGS = ["-l:libstdc++.so.6"]
+
 EXTENSIONS = [
     CUDAExtension(
         name="h3_a100._C",
         sources=[os.path.join(ROOT, s) for s in SOURCES],
         include_dirs=[os.path.join(ROOT, "csrc")],
         extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+        extra_link_args=LINK_FLAGS,
     )
 ]
 # H3_CHECKED_BUILD=1 also builds h3_a100._C_checked: the same kernels with
@@ -60,6 +66,7 @@ if os.environ.get("H3_CHECKED_BUILD", "0") == "1":
             include_dirs=[os.path.join(ROOT, "csrc")],
             extra_compile_args={"cxx": ["-O3", "-std=c++17", "-DH3_BOUNDS_CHECK"],
                                 "nvcc": NVCC_FLAGS + ["-DH3_BOUNDS_CHECK"]},
+            extra_link_args=LINK_FLAGS,
         )
     )
 
