@@ -1,0 +1,866 @@
+// Attention over packed sequences, backward, on tcgen05 (sm_100a).
+//
+//   p = 2^(scale log2e q k^T - lse2),  dp = do v^T,  ds = p (dp - delta),  delta = sum_d o do
+//   dq = scale ds k,  dk = scale ds^T q,  dv = p^T do     (dk, dv summed over the heads of a group)
+//
+// Three launches and no atomics, so results do not depend on the order of blocks:
+//   delta   delta and lse2 per row, laid out [Hk, Tq, G] as the rows of the query tiles
+//   dq      one 128-row query tile per item, loop over key tiles:   S, dP -> dS -> dQ += dS K
+//   dkv     one 128-key tile per item, loop over query tiles:       S^T, dP^T -> P^T, dS^T ->
+//           dV += P^T dO, dK += dS^T Q; the heads of a group are rows of the query tiles, so their
+//           sum is part of the accumulation
+// S and dP are computed twice (7 products instead of 5).  The alternative, one
+// kernel that adds dQ tiles into global memory, needs an fp32 dQ buffer, a
+// zero fill and a conversion pass, gives sums in no fixed order, and its S -> dS -> dQ
+// -> reduce chain leaves the tensor core idle for half of each step.  Here the
+// chain is short enough to overlap: S of the next step is issued as soon as
+// this step's S is in registers, so the exponentials run beside the products.
+//
+// Both kernels are persistent over a host-balanced list (packed.h), 384 threads:
+// warp 0 TMA loads, warp 1 issues the MMAs, warp 2 zeroes tile rows past a
+// sequence (they belong to the next one and 0 * NaN would leak into the sums),
+// warp 3 (dkv) stages lse2 and delta of the query tile, warps 4..11 softmax:
+// one row a thread, the two warpgroups take 64 columns each.
+// P and dS are rounded to bf16 (the MMA's operand type); all sums are fp32.
+// TMEM columns: dq   dQ [0,128)  S [128,256)  dP, dS two buffers [256,512)
+//               dkv  dV [0,128)  dK [128,256)  S^T [256,384)  dP^T, then P^T and dS^T [384,512)
+// Every wait is bounded (ptx.cuh); every TMA load targets one CTA only.
+#include "../common/ptx.cuh"
+#include "packed.h"
+#include "tile.cuh"
+
+#include <cmath>
+
+namespace h3 {
+namespace {
+
+constexpr int kThreads = 384;
+// Register split (setmaxnreg): 384 x 168 at launch = 128 x 72 + 256 x 216.
+constexpr int kLaunchRegs = 168, kRegsLow = 72, kRegsHigh = 216;
+static_assert(128 * kRegsLow + 256 * kRegsHigh == kThreads * kLaunchRegs, "register split");
+
+template <int D>
+struct Bwd {
+  static constexpr int kChunks = D / 64;
+  static constexpr int kTile = kChunks * kChunkBytes;
+  // Two resident tiles, a ring of three (read by two products, a step apart) and a ring of two.
+  static constexpr int kLong = 3, kShort = 2;
+  static constexpr int kTiles = 2 + kLong + kShort;
+  static constexpr int kExtra = 2 * 2 * 128 * 4 + 512;   // two stages of lse2 and delta, barriers
+  static constexpr int kSmem = kTiles * kTile + kExtra;
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+__device__ __forceinline__ PackedItem load_item(const PackedItem* p) {
+  PackedItem it;
+  const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
+  it.q0 = a.x, it.nq = a.y, it.k0 = a.z, it.nk = a.w, it.diag = b.x, it.head = b.y, it.slot = b.z, it.pad = b.w;
+  return it;
+}
+
+// A ring of tiles.  A tile whose last rows must be zeroed arrives on tail[slot];
+// the cleaning warp then makes the arrival on full[slot].
+template <int SLOTS>
+struct Ring {
+  uint64_t *full, *empty, *tail;
+  uint8_t* base;
+  static constexpr int kBarriers = 3 * SLOTS;
+  __device__ __forceinline__ void place(uint64_t* bars, uint8_t* tiles) {
+    full = bars, empty = bars + SLOTS, tail = bars + 2 * SLOTS, base = tiles;
+  }
+  __device__ __forceinline__ void init() const {
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&tail[s], 1);
+    }
+  }
+  __device__ __forceinline__ static int slot(int n) { return n % SLOTS; }
+  __device__ __forceinline__ bool wait_full(int n, uint64_t limit, volatile int* abort) const {
+    return mbar_wait(&full[n % SLOTS], static_cast<uint32_t>(n / SLOTS) & 1u, limit, abort);
+  }
+};
+
+// The loader's side of a ring.
+template <int SLOTS>
+struct Feed {
+  int n = 0;
+  uint32_t tail_slots = 0, tail_parity = 0;
+  // Waits for the next slot and arms its barrier; null if the wait gave up.
+  __device__ __forceinline__ uint64_t* next(const Ring<SLOTS>& r, bool tail, uint32_t bytes, uint64_t limit,
+                                            volatile int* abort, int& slot) {
+    slot = n % SLOTS;
+    if (!mbar_wait(&r.empty[slot], (static_cast<uint32_t>(n / SLOTS) & 1u) ^ 1u, limit, abort)) return nullptr;
+    uint64_t* full = tail ? &r.tail[slot] : &r.full[slot];
+    tail_slots = (tail_slots & ~(1u << slot)) | (tail ? 1u << slot : 0u);
+    if (tail) tail_parity ^= 1u << slot;
+    mbar_arrive_expect_tx(full, bytes);
+    ++n;
+    return full;
+  }
+  // Never leave a TMA write in flight into this CTA's shared memory.
+  __device__ __forceinline__ void drain(const Ring<SLOTS>& r, uint64_t limit) const {
+    volatile int never = 0;
+    for (int s = 0; s < min(n, SLOTS); ++s) {
+      const int last = (n - 1 - s) / SLOTS * SLOTS + s;
+      if (tail_slots >> s & 1u)
+        mbar_wait(&r.tail[s], (tail_parity >> s & 1u) ^ 1u, limit, &never);
+      else
+        mbar_wait(&r.full[s], static_cast<uint32_t>(last / SLOTS) & 1u, limit, &never);
+    }
+  }
+};
+
+// One tail tile of a ring (all lanes of the cleaning warp).
+template <int CHUNKS, int TILE, int SLOTS>
+__device__ __forceinline__ bool clean_tile(const Ring<SLOTS>& r, int n, int first, uint32_t& parity, uint64_t limit,
+                                           volatile int* abort) {
+  const int slot = n % SLOTS;
+  if (!__all_sync(0xffffffffu, mbar_wait(&r.tail[slot], parity >> slot & 1u, limit, abort))) return false;
+  parity ^= 1u << slot;
+  zero_tile_rows<CHUNKS>(r.base + slot * TILE, first);
+  fence_async_smem();
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(&r.full[slot]);
+  return true;
+}
+
+// S-shaped product of two K-major tiles: D[tmem] = A B^T over D columns.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, const uint8_t* a, const uint8_t* b) {
+  constexpr uint32_t kIdesc = umma_idesc_bf16(128, 128, false, false);
+  const uint32_t sa = smem_u32(a), sb = smem_u32(b);
+#pragma unroll
+  for (int ds = 0; ds < D / 16; ++ds) {
+    const uint32_t off = (ds >> 2) * kChunkBytes + (ds & 3) * 32;
+    umma_f16_ss(d_tmem, umma_smem_desc(sa + off, 16, 1024), umma_smem_desc(sb + off, 16, 1024), kIdesc,
+                ds > 0 ? 1u : 0u);
+  }
+}
+
+// Accumulating product with the left operand in TMEM (packed bf16; eight
+// columns per 16 of K, the second half of K at column `half`) and an MN-major tile.
+template <int D>
+__device__ __forceinline__ void issue_accum(uint32_t d_tmem, uint32_t a_tmem, uint32_t half, const uint8_t* b,
+                                            bool first) {
+  constexpr uint32_t kIdesc = umma_idesc_bf16(128, D, false, true);
+  const uint32_t sb = smem_u32(b);
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+    umma_f16_ts(d_tmem, a_tmem + (ks >> 2) * half + (ks & 3) * 8, umma_smem_desc(sb + ks * 2048, kChunkBytes, 1024),
+                kIdesc, (!first || ks > 0) ? 1u : 0u);
+}
+
+// COLS TMEM columns of this thread's row -> bf16 row in global memory.
+template <int COLS>
+__device__ __forceinline__ void store_row(uint32_t taddr, bool any, float scale, __nv_bfloat16* out, long off, bool live,
+                                          long extent, const KernelStatus& st) {
+#pragma unroll
+  for (int c = 0; c < COLS / 16; ++c) {
+    uint32_t r[16];
+    if (any) {
+      tmem_ld16(taddr + c * 16, r);
+      tmem_ld_wait();
+    }
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = any ? __uint_as_float(r[k]) * scale : 0.f;
+    const long first = off + c * 16;
+    if (!live || !H3_IN_BOUNDS(first, first + 15, extent, st)) continue;
+    uint4* dst = reinterpret_cast<uint4*>(out + first);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      dst[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                          pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+  }
+}
+
+__device__ __forceinline__ void give_up(const KernelStatus& st, volatile int* abort, int code, int detail) {
+  report_status(st, code, detail);
+  *abort = 1;
+}
+
+// ---------------------------------------------------------------- delta
+// delta = sum_d o do and lse2 = lse log2(e) (+inf where the row sees no key, so
+// that 2^(s - lse2) = 0), both [Hk, Tq, G].  D / 8 lanes per row.
+template <int D>
+__global__ void __launch_bounds__(256) packed_delta_kernel(PackedBwdParams p) {
+  constexpr int kLanes = D / 8;
+  const long item = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int l = threadIdx.x % kLanes;
+  const bool live = item < p.Tq * p.Hq;
+  const long t = live ? item / p.Hq : 0;
+  const int h = live ? static_cast<int>(item - t * p.Hq) : 0;
+  float s = 0.f;
+  if (live) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p.o + t * p.o_tok + h * p.o_head + l * 8));
+    const uint4 b = *reinterpret_cast<const uint4*>(p.dout + t * p.do_tok + h * p.do_head + l * 8);
+    const __nv_bfloat162* a2 = reinterpret_cast<const __nv_bfloat162*>(&a);
+    const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = __bfloat1622float2(a2[i]), y = __bfloat1622float2(b2[i]);
+      s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+    }
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (live && l == 0) {
+    const int kh = h / p.G, g = h - kh * p.G;
+    const long at = (kh * p.Tq + t) * p.G + g;
+    const float lse = p.lse[h * p.Tq + t];
+    p.delta[at] = s;
+    p.lse2[at] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+  }
+}
+
+// ---------------------------------------------------------------- dq
+struct DqBars {
+  uint64_t *q_full, *do_full, *q_empty, *do_empty, *s_full, *s_read, *dp_full, *ds_full, *dq_full, *drain;
+};
+
+// Key tiles of the item and live rows of the last one if it is cut short (else 0).
+__device__ __forceinline__ int key_tiles(const PackedItem& it, int& tail) {
+  const int seen = min(it.nk, max(0, it.nq + it.diag));
+  const int n = (seen + 127) >> 7;
+  const int left = it.nk - (n - 1) * 128;
+  tail = (n > 0 && left < 128) ? left : 0;
+  return n;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
+                     const __grid_constant__ PackedBwdParams p) {
+  using C = Bwd<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;
+  uint8_t* sDO = sQ + C::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kTiles * C::kTile);
+  Ring<C::kLong> rk;
+  Ring<C::kShort> rv;
+  rk.place(bars, sDO + C::kTile);
+  rv.place(bars + rk.kBarriers, rk.base + C::kLong * C::kTile);
+  DqBars b;
+  uint64_t* nb = bars + rk.kBarriers + rv.kBarriers;
+  b.q_full = nb, b.do_full = nb + 1, b.q_empty = nb + 2, b.do_empty = nb + 3, b.s_full = nb + 4, b.s_read = nb + 5;
+  b.dp_full = nb + 6, b.ds_full = nb + 8, b.dq_full = nb + 9, b.drain = nb + 10;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 11);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = warp_id();
+  const uint64_t limit = p.status.limit_ns;
+  if (threadIdx.x == 0) {
+    rk.init();
+    rv.init();
+    for (int i = 0; i < 11; ++i) mbar_init(nb + i, (nb + i == b.s_read || nb + i == b.ds_full) ? 256 : 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tq);
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+    tma_prefetch_desc(&tdo);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int begin = p.begin[blockIdx.x], end = p.begin[blockIdx.x + 1];
+  if (warp < 4) {
+    setmaxnreg_dec<kRegsLow>();
+    if (warp == 0 && elect_one()) {
+      const uint32_t q_bytes = static_cast<uint32_t>(p.bt * p.G) * 128u * C::kChunks;
+      Feed<C::kLong> fk;
+      Feed<C::kShort> fv;
+      int q_used = 0, do_used = 0;
+      bool ok = true;
+      for (int i = begin; i < end && ok; ++i) {
+        const PackedItem it = load_item(p.items + i);
+        int tail;
+        const int n = key_tiles(it, tail);
+        if (n == 0) continue;
+        int slot;
+        auto load_q = [&](uint64_t* full, const CUtensorMap* map, uint8_t* dst) {
+          mbar_arrive_expect_tx(full, q_bytes);
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+            tma_load_4d(dst + c * kChunkBytes, map, full, c * 64, 0, it.head, it.q0);
+        };
+        ok = mbar_wait(b.q_empty, (q_used & 1) ^ 1u, limit, abort_flag);
+        if (!ok) break;
+        load_q(b.q_full, &tq, sQ);
+        ++q_used;
+        for (int j = 0; j < n && ok; ++j) {
+          uint64_t* full = fk.next(rk, tail != 0 && j == n - 1, C::kTile, limit, abort_flag, slot);
+          if (full != nullptr)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_3d(rk.base + slot * C::kTile + c * kChunkBytes, &tk, full, c * 64, it.head, it.k0 + j * 128);
+          ok = full != nullptr;
+          if (ok && j == 0) {
+            ok = mbar_wait(b.do_empty, (do_used & 1) ^ 1u, limit, abort_flag);
+            if (ok) {
+              load_q(b.do_full, &tdo, sDO);
+              ++do_used;
+            }
+          }
+          if (!ok) break;
+          full = fv.next(rv, false, C::kTile, limit, abort_flag, slot);
+          if (full != nullptr)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_3d(rv.base + slot * C::kTile + c * kChunkBytes, &tv, full, c * 64, it.head, it.k0 + j * 128);
+          ok = full != nullptr;
+        }
+      }
+      if (!ok) give_up(p.status, abort_flag, kStatusTimeoutEmpty, fk.n);
+      fk.drain(rk, limit);
+      fv.drain(rv, limit);
+      volatile int never = 0;
+      if (q_used > 0) mbar_wait(b.q_full, (q_used - 1) & 1, limit, &never);
+      if (do_used > 0) mbar_wait(b.do_full, (do_used - 1) & 1, limit, &never);
+    } else if (warp == 1 && elect_one()) {
+      int nk = 0, nv = 0, items = 0, st = 0;
+      bool ok = true, any = false;
+      for (int i = begin; i < end && ok; ++i) {
+        const PackedItem it = load_item(p.items + i);
+        int tail;
+        const int n = key_tiles(it, tail);
+        if (n == 0) continue;
+        auto scores = [&](int j) {
+          if (!rk.wait_full(nk + j, limit, abort_flag)) return false;
+          tc_fence_after();
+          issue_scores<D>(tmem + 128, sQ, rk.base + rk.slot(nk + j) * C::kTile);
+          umma_commit(b.s_full);
+          if (j + 1 == n) umma_commit(b.q_empty);
+          any = true;
+          return true;
+        };
+        auto grads = [&](int j) {
+          if (!rv.wait_full(nv + j, limit, abort_flag)) return false;
+          tc_fence_after();
+          issue_scores<D>(tmem + 256 + ((st + j) & 1) * 128, sDO, rv.base + rv.slot(nv + j) * C::kTile);
+          umma_commit(&b.dp_full[(st + j) & 1]);
+          umma_commit(&rv.empty[rv.slot(nv + j)]);
+          if (j + 1 == n) umma_commit(b.do_empty);
+          return true;
+        };
+        ok = mbar_wait(b.q_full, items & 1, limit, abort_flag) && scores(0) &&
+             mbar_wait(b.do_full, items & 1, limit, abort_flag) && grads(0);
+        for (int j = 0; j < n && ok; ++j) {
+          if (j + 1 < n) {
+            ok = mbar_wait(b.s_read, (st + j) & 1, limit, abort_flag) && scores(j + 1) && grads(j + 1);
+            if (!ok) break;
+          }
+          ok = mbar_wait(b.ds_full, (st + j) & 1, limit, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_accum<D>(tmem, tmem + 256 + ((st + j) & 1) * 128, 64, rk.base + rk.slot(nk + j) * C::kTile, j == 0);
+          umma_commit(&rk.empty[rk.slot(nk + j)]);
+          if (j + 1 == n) umma_commit(b.dq_full);
+        }
+        nk += n, nv += n, st += n;
+        ++items;
+      }
+      if (!ok) give_up(p.status, abort_flag, kStatusTimeoutFull, nk);
+      if (any) {
+        umma_commit(b.drain);
+        volatile int never = 0;
+        mbar_wait(b.drain, 0, limit, &never);
+      }
+    } else if (warp == 2) {
+      int nk = 0;
+      uint32_t parity = 0;
+      for (int i = begin; i < end; ++i) {
+        const PackedItem it = load_item(p.items + i);
+        int tail;
+        const int n = key_tiles(it, tail);
+        if (tail != 0 && !clean_tile<C::kChunks, C::kTile>(rk, nk + n - 1, tail, parity, limit, abort_flag)) {
+          if (lane_id() == 0) give_up(p.status, abort_flag, kStatusTimeoutFull, i);
+          break;
+        }
+        nk += n;
+      }
+    }
+    __syncwarp();
+    tc_fence_before();
+    named_bar_sync(1, kThreads);
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, 512);
+    }
+    return;
+  }
+  setmaxnreg_inc<kRegsHigh>();
+  // ---------------------------------------------------------- softmax warps
+  const int wg = (warp - 4) >> 2;
+  const int row = (warp & 3) * 32 + lane_id();
+  const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t tS = tmem + 128 + wg * 64 + lane_off;
+  const int tok = row / p.G, g = row - tok * p.G;
+  int st = 0, items = 0;
+  bool ok = true;
+  for (int i = begin; i < end; ++i) {
+    const PackedItem it = load_item(p.items + i);
+    int tail;
+    const int n = key_tiles(it, tail);
+    const bool live = row < it.nq * p.G;
+    const int seen = live ? min(it.nk, max(0, tok + it.diag + 1)) : it.nk;
+    const long q = static_cast<long>(it.q0) + tok;
+    float lse2 = INFINITY, delta = 0.f;
+    if (live) {
+      const long at = (it.head * p.Tq + q) * p.G + g;
+      lse2 = p.lse2[at];
+      delta = p.delta[at];
+    }
+    const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), neg_lse = pack2(-lse2, -lse2);
+    const uint64_t neg_delta = pack2(-delta, -delta);
+    for (int j = 0; j < n; ++j, ++st) {
+      const uint32_t tP = tmem + 256 + (st & 1) * 128 + wg * 64 + lane_off;
+      ok = __all_sync(0xffffffffu, mbar_wait(b.s_full, st & 1, limit, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[2][32];
+      tmem_ld32(tS, s[0]);
+      tmem_ld32(tS + 32, s[1]);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(b.s_read);
+      const int valid = seen - j * 128 - wg * 64;
+      const bool cut = __any_sync(0xffffffffu, valid < 64);
+      uint64_t pr[2][16];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float x, y;
+          unpack2(fma2(pack2(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), scale2, neg_lse), x, y);
+          pr[c][k] = pack2(ex2(x), ex2(y));
+        }
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.dp_full[st & 1], (st >> 1) & 1, limit, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t packed[2][16];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t dp[32];
+        tmem_ld32(tP + c * 32, dp);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float x, y;
+          unpack2(mul2(pr[c][k], add2(pack2(__uint_as_float(dp[2 * k]), __uint_as_float(dp[2 * k + 1])), neg_delta)), x,
+                  y);
+          if (cut) {   // a select, not a product: what a masked place holds may be NaN
+            x = c * 32 + 2 * k < valid ? x : 0.f;
+            y = c * 32 + 2 * k + 1 < valid ? y : 0.f;
+          }
+          packed[c][k] = pack_bf16x2(x, y);
+        }
+      }
+      // dS over this warpgroup's own, already read dP columns.
+      tmem_st16(tP, packed[0]);
+      tmem_st16(tP + 16, packed[1]);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(b.ds_full);
+    }
+    if (ok && n > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(b.dq_full, items & 1, limit, abort_flag));
+      ++items;
+    }
+    if (!ok) break;
+    tc_fence_after();
+    const int head = it.head * p.G + g, half = wg * (D / 2);
+    store_row<D / 2>(tmem + half + lane_off, n > 0, p.scale, p.dq, q * p.dq_tok + head * p.dq_head + half, live,
+                     p.dq_extent, p.status);
+    tc_fence_before();
+  }
+  if (!ok && lane_id() == 0) give_up(p.status, abort_flag, kStatusTimeoutAccFull, st);
+  __syncwarp();
+  tc_fence_before();
+  named_bar_sync(1, kThreads);
+}
+
+// ---------------------------------------------------------------- dk, dv
+struct DkvBars {
+  uint64_t *k_full, *v_full, *kv_empty, *s_full, *s_read, *dp_full, *ds_full, *acc_full, *row_full, *drain;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_dkv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
+                      const __grid_constant__ PackedBwdParams p) {
+  using C = Bwd<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + C::kTile;
+  float* sRow = reinterpret_cast<float*>(smem + C::kTiles * C::kTile);   // [2][lse2 128 | delta 128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + 2 * 256);
+  Ring<C::kLong> rq;
+  Ring<C::kShort> rd;
+  rq.place(bars, sV + C::kTile);
+  rd.place(bars + rq.kBarriers, rq.base + C::kLong * C::kTile);
+  DkvBars b;
+  uint64_t* nb = bars + rq.kBarriers + rd.kBarriers;
+  b.k_full = nb, b.v_full = nb + 1, b.kv_empty = nb + 2, b.s_full = nb + 3, b.s_read = nb + 4, b.dp_full = nb + 5;
+  b.ds_full = nb + 6, b.acc_full = nb + 7, b.row_full = nb + 8, b.drain = nb + 10;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 11);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = warp_id();
+  const uint64_t limit = p.status.limit_ns;
+  const int rows_full = p.bt * p.G;      // rows of a whole query tile
+  if (threadIdx.x == 0) {
+    rq.init();
+    rd.init();
+    for (int i = 0; i < 11; ++i) mbar_init(nb + i, (nb + i == b.s_read || nb + i == b.ds_full) ? 256 : 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tq);
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+    tma_prefetch_desc(&tdo);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp >= 4 && rows_full < 128) {
+    // Rows that no load writes (128 is not a multiple of the group): zero once.
+    for (int s = warp - 4; s < C::kLong + C::kShort; s += 8)
+      zero_tile_rows<C::kChunks>(rq.base + s * C::kTile, rows_full);
+    fence_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int begin = p.begin[blockIdx.x], end = p.begin[blockIdx.x + 1];
+  // Query tiles of an item and live rows of the last one.
+  auto query_tiles = [&](const PackedItem& it, int& last_rows) {
+    const int n = (it.nq + p.bt - 1) / p.bt;
+    last_rows = (it.nq - (n - 1) * p.bt) * p.G;
+    return n;
+  };
+  if (warp < 4) {
+    setmaxnreg_dec<kRegsLow>();
+    if (warp == 0 && elect_one()) {
+      const uint32_t q_bytes = static_cast<uint32_t>(rows_full) * 128u * C::kChunks;
+      Feed<C::kLong> fq;
+      Feed<C::kShort> fd;
+      int used = 0;
+      bool ok = true;
+      for (int i = begin; i < end && ok; ++i) {
+        const PackedItem it = load_item(p.items + i);
+        int last_rows, slot;
+        const int n = query_tiles(it, last_rows);
+        if (n == 0) continue;
+        ok = mbar_wait(b.kv_empty, (used & 1) ^ 1u, limit, abort_flag);
+        if (!ok) break;
+        ++used;
+        mbar_arrive_expect_tx(b.k_full, C::kTile);
+        mbar_arrive_expect_tx(b.v_full, C::kTile);
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c)
+          tma_load_3d(sK + c * kChunkBytes, &tk, b.k_full, c * 64, it.head, it.k0);
+        for (int j = 0; j < n && ok; ++j) {
+          const bool tail = j == n - 1 && last_rows < rows_full;
+          const int q = it.q0 + j * p.bt;
+          uint64_t* full = fq.next(rq, tail, q_bytes, limit, abort_flag, slot);
+          if (full != nullptr)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_4d(rq.base + slot * C::kTile + c * kChunkBytes, &tq, full, c * 64, 0, it.head, q);
+          if (j == 0)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_3d(sV + c * kChunkBytes, &tv, b.v_full, c * 64, it.head, it.k0);
+          ok = full != nullptr;
+          if (!ok) break;
+          full = fd.next(rd, tail, q_bytes, limit, abort_flag, slot);
+          if (full != nullptr)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_4d(rd.base + slot * C::kTile + c * kChunkBytes, &tdo, full, c * 64, 0, it.head, q);
+          ok = full != nullptr;
+        }
+      }
+      if (!ok) give_up(p.status, abort_flag, kStatusTimeoutEmpty, fq.n);
+      fq.drain(rq, limit);
+      fd.drain(rd, limit);
+      volatile int never = 0;
+      if (used > 0) {
+        mbar_wait(b.k_full, (used - 1) & 1, limit, &never);
+        mbar_wait(b.v_full, (used - 1) & 1, limit, &never);
+      }
+    } else if (warp == 1 && elect_one()) {
+      int nt = 0, items = 0;    // query tiles (= steps) so far
+      bool ok = true, any = false;
+      for (int i = begin; i < end && ok; ++i) {
+        const PackedItem it = load_item(p.items + i);
+        int last_rows;
+        const int n = query_tiles(it, last_rows);
+        if (n == 0) continue;
+        auto scores = [&](int j) {
+          if (!rq.wait_full(nt + j, limit, abort_flag)) return false;
+          tc_fence_after();
+          issue_scores<D>(tmem + 256, sK, rq.base + rq.slot(nt + j) * C::kTile);
+          umma_commit(b.s_full);
+          any = true;
+          return true;
+        };
+        auto grads = [&](int j) {
+          if (!rd.wait_full(nt + j, limit, abort_flag)) return false;
+          tc_fence_after();
+          issue_scores<D>(tmem + 384, sV, rd.base + rd.slot(nt + j) * C::kTile);
+          umma_commit(b.dp_full);
+          return true;
+        };
+        ok = mbar_wait(b.k_full, items & 1, limit, abort_flag) && scores(0) &&
+             mbar_wait(b.v_full, items & 1, limit, abort_flag) && grads(0);
+        for (int j = 0; j < n && ok; ++j) {
+          if (j + 1 < n) {
+            ok = mbar_wait(b.s_read, (nt + j) & 1, limit, abort_flag) && scores(j + 1);
+            if (!ok) break;
+          }
+          ok = mbar_wait(b.ds_full, (nt + j) & 1, limit, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          // P^T of the two warpgroups at columns 384 and 448, dS^T at 416 and 480.
+          issue_accum<D>(tmem, tmem + 384, 64, rd.base + rd.slot(nt + j) * C::kTile, j == 0);
+          umma_commit(&rd.empty[rd.slot(nt + j)]);
+          issue_accum<D>(tmem + 128, tmem + 416, 64, rq.base + rq.slot(nt + j) * C::kTile, j == 0);
+          umma_commit(&rq.empty[rq.slot(nt + j)]);
+          if (j + 1 < n) {
+            ok = grads(j + 1);
+          } else {
+            umma_commit(b.acc_full);
+            umma_commit(b.kv_empty);
+          }
+        }
+        nt += n;
+        ++items;
+      }
+      if (!ok) give_up(p.status, abort_flag, kStatusTimeoutFull, nt);
+      if (any) {
+        umma_commit(b.drain);
+        volatile int never = 0;
+        mbar_wait(b.drain, 0, limit, &never);
+      }
+    } else if (warp == 2) {
+      int nt = 0;
+      uint32_t pq = 0, pd = 0;
+      for (int i = begin; i < end; ++i) {
+        const PackedItem it = load_item(p.items + i);
+        int last_rows;
+        const int n = query_tiles(it, last_rows);
+        if (n > 0 && last_rows < rows_full &&
+            (!clean_tile<C::kChunks, C::kTile>(rq, nt + n - 1, last_rows, pq, limit, abort_flag) ||
+             !clean_tile<C::kChunks, C::kTile>(rd, nt + n - 1, last_rows, pd, limit, abort_flag))) {
+          if (lane_id() == 0) give_up(p.status, abort_flag, kStatusTimeoutFull, i);
+          break;
+        }
+        nt += n;
+      }
+    } else if (warp == 3) {
+      // lse2 and delta of each query tile; rows past the tile's tokens weigh nothing.
+      int st = 0;
+      bool ok = true;
+      for (int i = begin; i < end && ok; ++i) {
+        const PackedItem it = load_item(p.items + i);
+        int last_rows;
+        const int n = query_tiles(it, last_rows);
+        for (int j = 0; j < n; ++j, ++st) {
+          const int rows = j == n - 1 ? last_rows : rows_full;
+          const long at = (it.head * p.Tq + it.q0 + static_cast<long>(j) * p.bt) * p.G;
+          float a[4], d[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = k * 32 + lane_id();
+            a[k] = r < rows ? p.lse2[at + r] : INFINITY;
+            d[k] = r < rows ? p.delta[at + r] : 0.f;
+          }
+          // The stage is free once the step before last has been used up.
+          ok = __all_sync(0xffffffffu, st < 2 || mbar_wait(b.ds_full, st & 1, limit, abort_flag));
+          if (!ok) break;
+          float* dst = sRow + (st & 1) * 256;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            dst[k * 32 + lane_id()] = a[k];
+            dst[128 + k * 32 + lane_id()] = d[k];
+          }
+          __syncwarp();
+          if (lane_id() == 0) mbar_arrive(&b.row_full[st & 1]);
+        }
+      }
+      if (!ok && lane_id() == 0) give_up(p.status, abort_flag, kStatusTimeoutEmpty, st);
+    }
+    __syncwarp();
+    tc_fence_before();
+    named_bar_sync(1, kThreads);
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, 512);
+    }
+    return;
+  }
+  setmaxnreg_inc<kRegsHigh>();
+  // ---------------------------------------------------------- softmax warps
+  const int wg = (warp - 4) >> 2;
+  const int row = (warp & 3) * 32 + lane_id();       // key of the tile
+  const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t tS = tmem + 256 + wg * 64 + lane_off, tP = tmem + 384 + wg * 64 + lane_off;
+  const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+  int st = 0, items = 0;
+  bool ok = true;
+  for (int i = begin; i < end; ++i) {
+    const PackedItem it = load_item(p.items + i);
+    int last_rows;
+    const int n = query_tiles(it, last_rows);
+    for (int j = 0; j < n; ++j, ++st) {
+      const float* rs = sRow + (st & 1) * 256 + wg * 64;
+      ok = __all_sync(0xffffffffu, mbar_wait(b.s_full, st & 1, limit, abort_flag) &&
+                                       mbar_wait(&b.row_full[st & 1], (st >> 1) & 1, limit, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[2][32];
+      tmem_ld32(tS, s[0]);
+      tmem_ld32(tS + 32, s[1]);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(b.s_read);
+      // Columns are token * G + head: the tokens before key - diag do not see this key.
+      const int hidden = max(0, row - it.diag - j * p.bt) * p.G - wg * 64;
+      const bool cut = __any_sync(0xffffffffu, hidden > 0);
+      uint64_t pr[2][16];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float4 l = *reinterpret_cast<const float4*>(rs + c * 32 + 4 * k);
+          float x, y, z, w;
+          unpack2(fma2(pack2(__uint_as_float(s[c][4 * k]), __uint_as_float(s[c][4 * k + 1])), scale2, pack2(-l.x, -l.y)),
+                  x, y);
+          unpack2(fma2(pack2(__uint_as_float(s[c][4 * k + 2]), __uint_as_float(s[c][4 * k + 3])), scale2,
+                       pack2(-l.z, -l.w)),
+                  z, w);
+          x = ex2(x), y = ex2(y), z = ex2(z), w = ex2(w);
+          if (cut) {
+            const int at = c * 32 + 4 * k;
+            x = at < hidden ? 0.f : x;
+            y = at + 1 < hidden ? 0.f : y;
+            z = at + 2 < hidden ? 0.f : z;
+            w = at + 3 < hidden ? 0.f : w;
+          }
+          pr[c][2 * k] = pack2(x, y);
+          pr[c][2 * k + 1] = pack2(z, w);
+        }
+      ok = __all_sync(0xffffffffu, mbar_wait(b.dp_full, st & 1, limit, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t dp[2][32];
+      tmem_ld32(tP, dp[0]);
+      tmem_ld32(tP + 32, dp[1]);
+      tmem_ld_wait();
+      // This warpgroup's dP columns are read: P^T goes over the first half of them, dS^T over the second.
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pp[16], pd[16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float4 d = *reinterpret_cast<const float4*>(rs + 128 + c * 32 + 4 * k);
+          float x, y, z, w;
+          unpack2(pr[c][2 * k], x, y);
+          unpack2(pr[c][2 * k + 1], z, w);
+          pp[2 * k] = pack_bf16x2(x, y);
+          pp[2 * k + 1] = pack_bf16x2(z, w);
+          unpack2(mul2(pr[c][2 * k], add2(pack2(__uint_as_float(dp[c][4 * k]), __uint_as_float(dp[c][4 * k + 1])),
+                                          pack2(-d.x, -d.y))),
+                  x, y);
+          unpack2(mul2(pr[c][2 * k + 1], add2(pack2(__uint_as_float(dp[c][4 * k + 2]), __uint_as_float(dp[c][4 * k + 3])),
+                                              pack2(-d.z, -d.w))),
+                  z, w);
+          if (cut) {   // a select, not a product: what a masked place holds may be NaN
+            const int at = c * 32 + 4 * k;
+            x = at < hidden ? 0.f : x;
+            y = at + 1 < hidden ? 0.f : y;
+            z = at + 2 < hidden ? 0.f : z;
+            w = at + 3 < hidden ? 0.f : w;
+          }
+          pd[2 * k] = pack_bf16x2(x, y);
+          pd[2 * k + 1] = pack_bf16x2(z, w);
+        }
+        tmem_st16(tP + c * 16, pp);
+        tmem_st16(tP + 32 + c * 16, pd);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(b.ds_full);
+    }
+    if (ok && n > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(b.acc_full, items & 1, limit, abort_flag));
+      ++items;
+    }
+    if (!ok) break;
+    tc_fence_after();
+    const bool live = row < it.nk;
+    const long key = static_cast<long>(it.k0) + row;
+    if (wg == 0)
+      store_row<D>(tmem + lane_off, n > 0, 1.f, p.dv, key * p.dv_tok + it.head * p.dv_head, live, p.dv_extent, p.status);
+    else
+      store_row<D>(tmem + 128 + lane_off, n > 0, p.scale, p.dk, key * p.dk_tok + it.head * p.dk_head, live,
+                   p.dk_extent, p.status);
+    tc_fence_before();
+  }
+  if (!ok && lane_id() == 0) give_up(p.status, abort_flag, kStatusTimeoutAccFull, st);
+  __syncwarp();
+  tc_fence_before();
+  named_bar_sync(1, kThreads);
+}
+
+template <int D>
+const char* configure() {
+  cudaFuncAttributes attr{};
+  auto one = [&](auto kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Bwd<D>::kSmem) == cudaSuccess &&
+           cudaFuncGetAttributes(&attr, kernel) == cudaSuccess && attr.numRegs == kLaunchRegs;
+  };
+  // setmaxnreg.inc waits for registers that the producer warpgroup releases:
+  // it only balances if the launch count is the assumed one.
+  if (!one(packed_dq_kernel<D>) || !one(packed_dkv_kernel<D>))
+    return "packed attention backward: cannot configure (the register split assumes 168 per thread)";
+  return nullptr;
+}
+
+}  // namespace
+
+const char* packed_bwd_configure() {
+  const char* e = configure<64>();
+  return e != nullptr ? e : configure<128>();
+}
+
+void launch_packed_delta(int head_dim, const PackedBwdParams& p, cudaStream_t stream) {
+  const long threads = p.Tq * p.Hq * (head_dim / 8);
+  const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+  if (head_dim == 128) packed_delta_kernel<128><<<blocks, 256, 0, stream>>>(p);
+  else packed_delta_kernel<64><<<blocks, 256, 0, stream>>>(p);
+}
+
+void launch_packed_dq(int head_dim, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                      const CUtensorMap& dout, const PackedBwdParams& p, cudaStream_t stream) {
+  if (head_dim == 128) packed_dq_kernel<128><<<blocks, kThreads, Bwd<128>::kSmem, stream>>>(q, k, v, dout, p);
+  else packed_dq_kernel<64><<<blocks, kThreads, Bwd<64>::kSmem, stream>>>(q, k, v, dout, p);
+}
+
+void launch_packed_dkv(int head_dim, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                       const CUtensorMap& dout, const PackedBwdParams& p, cudaStream_t stream) {
+  if (head_dim == 128) packed_dkv_kernel<128><<<blocks, kThreads, Bwd<128>::kSmem, stream>>>(q, k, v, dout, p);
+  else packed_dkv_kernel<64><<<blocks, kThreads, Bwd<64>::kSmem, stream>>>(q, k, v, dout, p);
+}
+
+}  // namespace h3

@@ -2,9 +2,11 @@
 #include <torch/extension.h>
 
 #include "attn/attention.h"
+#include "attn/packed_api.h"
 #include "comm/p2p.h"
 #include "elementwise/elementwise.h"
 #include "gemm/gemm.h"
+#include "rope/qk_rope.h"
 
 namespace h3 {
 at::Tensor pinned_empty(int64_t numel, c10::ScalarType dtype);
@@ -19,6 +21,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_bwd", &h3::attention_bwd, "tcgen05 attention backward", py::arg("qkv"), py::arg("o"),
         py::arg("lse"), py::arg("dout"), py::arg("heads"), py::arg("head_dim"), py::arg("status"),
         py::arg("limit_ns"), py::arg("trace") = py::none());
+  m.def("packed_schedule", &h3::packed_schedule, "work lists of a packed batch");
+  m.def("attention_packed_fwd", &h3::attention_packed_fwd, "tcgen05 attention over packed sequences, forward");
+  m.def("attention_packed_bwd", &h3::attention_packed_bwd, "tcgen05 attention over packed sequences, backward");
+  m.def("qk_rope_fwd", &h3::qk_rope_fwd, "multi-axis rotation of q and k, with their norms if weights are given");
+  m.def("qk_norm_rope_bwd", &h3::qk_norm_rope_bwd, "gradients of the norm and rotation of q and k");
   m.def("p2p_all_gather", &h3::p2p_all_gather, "pull all-gather over peer memory");
   m.def("p2p_all_gather_ce", &h3::p2p_all_gather_ce, "all-gather over peer memory on the copy engines");
   m.def("lora_rs_adamw", &h3::lora_rs_adamw, "fused LoRA reduce-scatter + clip + AdamW + all-gather");

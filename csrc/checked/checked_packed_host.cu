@@ -1,0 +1,2 @@
+// The bounds-checked build of attn/packed_host.cu (module h3_a100._C_checked).
+#include "../attn/packed_host.cu"

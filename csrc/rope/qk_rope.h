@@ -1,0 +1,24 @@
+// Host API of the query/key norm and multi-axis rotation kernels (see qk_rope.cu).
+#pragma once
+#include <ATen/ATen.h>
+
+#include <vector>
+
+namespace h3 {
+
+// q [T, Hq, D], k [T, Hk, D] (bf16 or fp32; Hk may be 0) -> rotated {q, k}, contiguous.
+// With weights ([D], bf16 or fp32) every head is RMS-normalised and scaled first.
+// positions [T, A] fp32 and freqs [sum(pairs)] fp32 may be absent (no rotation).
+std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& q_weight,
+                                    const c10::optional<at::Tensor>& k_weight,
+                                    const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& freqs,
+                                    const std::vector<int64_t>& pairs, bool interleaved, bool inverse, double eps);
+
+// Gradients {dq, dk, dq_weight [D] fp32, dk_weight [D] fp32} of the normalising form.
+std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+                                         const at::Tensor& k_weight, const c10::optional<at::Tensor>& positions,
+                                         const c10::optional<at::Tensor>& freqs, const std::vector<int64_t>& pairs,
+                                         bool interleaved, const at::Tensor& dq_out, const at::Tensor& dk_out,
+                                         double eps);
+
+}  // namespace h3

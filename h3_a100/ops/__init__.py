@@ -12,9 +12,10 @@ from __future__ import annotations
 
 import torch
 
+from .packing import AxisRope, PackedPlan
 from .torch_kernels import GatedResidual, Rope, TorchKernels
 
-__all__ = ["GatedResidual", "Rope", "TorchKernels", "get_kernels"]
+__all__ = ["AxisRope", "GatedResidual", "PackedPlan", "Rope", "TorchKernels", "get_kernels"]
 
 
 def get_kernels(backend: str, device: torch.device):

@@ -13,7 +13,9 @@ tcgen05 GEMM (``csrc/gemm/gemm_tcgen05.cu``) with its epilogue fused:
 
 Norm/modulate, gate, RoPE-inverse, AdaLN projection, flow/DMD elementwise
 passes, sum-of-squares and AdamW are the kernels of
-``csrc/elementwise/elementwise.cu``; attention is ``csrc/attn``.
+``csrc/elementwise/elementwise.cu``; attention is ``csrc/attn``.  Packed batches:
+``rope_axes`` and ``qk_norm_rope`` are ``csrc/rope/qk_rope.cu``, attention
+over packed sequences is ``csrc/attn/packed_{fwd,bwd}.cu``.
 
 Importing this module without the compiled extension raises: on a GPU the
 native path never falls back silently.
@@ -30,6 +32,7 @@ except ImportError as exc:  # pragma: no cover - exercised only on broken instal
         "h3_a100._C (the sm_100a extension) is not built; run `python setup.py build_ext --inplace`"
     ) from exc
 
+from .packing import AxisRope, PackedPlan
 from .torch_kernels import GatedResidual, Rope
 
 EPI_BF16, EPI_GELU, EPI_ROPE = _C.EPI_BF16, _C.EPI_GELU, _C.EPI_ROPE
@@ -38,6 +41,20 @@ STATUS_NAMES = {1: "timeout waiting for a TMA stage", 2: "timeout waiting for a 
                 3: "timeout waiting for an accumulator", 4: "timeout waiting for the epilogue",
                 5: "timeout waiting for a peer GPU", 6: "bad argument",
                 7: "out-of-bounds access caught by the bounds-checked build"}
+
+
+def _heads16(t: torch.Tensor) -> torch.Tensor:
+    """``t [tokens, heads, D]`` itself if the kernels can read its layout, else a contiguous copy.
+
+    They need unit stride within a head and every head on a 16-byte boundary
+    (a vector load, a TMA row); an expanded (zero-stride) dimension has no such layout.
+    """
+    unit = 16 // t.element_size()
+    if t.dim() != 3 or t.numel() == 0:
+        return t
+    fits = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
+        t.shape[d] == 1 or (t.stride(d) > 0 and t.stride(d) % unit == 0) for d in (0, 1))
+    return t if fits else t.contiguous()
 
 
 def _num_sms(device: torch.device) -> int:
@@ -191,6 +208,68 @@ class NativeKernels:
         if lse is None:
             raise ValueError("the tcgen05 attention backward needs the forward's log-sum-exp rows")
         return self.C.attention_bwd(qkv, o, lse, do, int(heads), int(head_dim), self.status, self.limit_ns)
+
+    # ------------------------------------------------------------ packed sequences
+    @staticmethod
+    def _rope_args(rope: AxisRope | None):
+        if rope is None:
+            return None, None, [], True
+        return rope.positions, rope.freqs, list(rope.pairs), rope.interleaved
+
+    def rope_axes(self, q, k, rope: AxisRope, inverse: bool = False):
+        """Rotate every head of ``q`` and ``k`` (``k`` may be None); ``inverse`` turns gradients back."""
+        pos, freqs, pairs, inter = self._rope_args(rope)
+        both = self.C.qk_rope_fwd(_heads16(q), q[:, :0] if k is None else _heads16(k), None, None, pos, freqs, pairs,
+                                  inter, bool(inverse), 0.0)
+        return both[0], None if k is None else both[1]
+
+    def qk_norm_rope(self, q, k, q_weight, k_weight, rope: AxisRope | None = None, eps=1e-6):
+        """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``), then the rotation."""
+        pos, freqs, pairs, inter = self._rope_args(rope)
+        both = self.C.qk_rope_fwd(_heads16(q), _heads16(k), q_weight, k_weight, pos, freqs, pairs, inter, False,
+                                  float(eps))
+        return both[0], both[1]
+
+    def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6):
+        """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32."""
+        pos, freqs, pairs, inter = self._rope_args(rope)
+        return tuple(self.C.qk_norm_rope_bwd(_heads16(q), _heads16(k), q_weight, k_weight, pos, freqs, pairs, inter,
+                                             _heads16(dq), _heads16(dk), float(eps)))
+
+    def packed_plan(self, q_lens, k_lens=None, *, heads, kv_heads, head_dim, causal=False) -> PackedPlan:
+        """Work lists of a packed batch, uploaded once; every layer's forward and backward uses them."""
+        plan = PackedPlan.lengths(q_lens, k_lens, heads=heads, kv_heads=kv_heads, head_dim=head_dim, causal=causal)
+        blob, meta = self.C.packed_schedule(list(plan.q_lens), list(plan.k_lens), plan.heads, plan.kv_heads,
+                                            plan.head_dim, plan.causal, self.sms)
+        return PackedPlan(plan.q_lens, plan.k_lens, plan.heads, plan.kv_heads, plan.head_dim, plan.causal,
+                          blob.to(self.device), tuple(meta))
+
+    @staticmethod
+    def _packed_args(plan: PackedPlan, scale):
+        if plan.blob is None:
+            raise ValueError("the plan was not made by this kernel set's packed_plan")
+        return plan.blob, plan.meta, plan.head_dim ** -0.5 if scale is None else float(scale)
+
+    def attention_packed_fwd(self, q, k, v, plan: PackedPlan, scale=None):
+        """Attention of each sequence of a packed batch with itself -> (o, lse [heads, tokens] fp32).
+
+        bf16, head dim 64 or 128; see ``TorchKernels.attention_packed_fwd``.
+        """
+        blob, meta, scale = self._packed_args(plan, scale)
+        o, lse = self.C.attention_packed_fwd(_heads16(q), _heads16(k), _heads16(v), blob, meta, scale, self.status,
+                                             self.limit_ns)
+        return o, lse
+
+    def attention_packed_bwd(self, q, k, v, o, lse, do, plan: PackedPlan, scale=None, out=None):
+        """Gradients ``(dq, dk, dv)``; ``out``: three tensors (views are fine) to write them into.
+
+        The sums over the heads of a group and over query tiles run in a fixed
+        order: the same inputs give the same bits.
+        """
+        blob, meta, scale = self._packed_args(plan, scale)
+        return tuple(self.C.attention_packed_bwd(_heads16(q), _heads16(k), _heads16(v), _heads16(o), lse, _heads16(do),
+                                                 blob, meta, scale, self.status, self.limit_ns,
+                                                 [] if out is None else list(out)))
 
     # ------------------------------------------------------------ small projections
     def adaln_project(self, temb, w, b):

@@ -18,6 +18,9 @@ Conventions shared with the native kernels (``h3_a100/ops/native.py``):
   scale ``s = alpha/r`` is applied exactly once, in ``lora_down``
   (``U = s * x A^T``) and in ``lora_dyb`` (``dyb = s * dy B``); every other
   LoRA term uses those scaled tensors;
+* packed batches (``PackedPlan``) keep heads apart: ``[tokens, heads, head_dim]``
+  for q and o, ``[tokens, kv_heads, head_dim]`` for k and v, any token and head
+  strides (views of a fused projection are fine);
 * RoPE rotates interleaved pairs ``(2i, 2i+1)`` of every head with per-token
   tables ``cos, sin: [T, head_dim/2]`` (fp32).
 """
@@ -29,6 +32,8 @@ from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
+
+from .packing import AxisRope, PackedPlan
 
 GELU_C = math.sqrt(2.0 / math.pi)
 
@@ -220,6 +225,140 @@ class TorchKernels:
             out = out.transpose(0, 1).reshape(qkv.shape[0], heads * head_dim)
             (dqkv,) = torch.autograd.grad(out, qkv_, do)
         return dqkv
+
+    # ---------------- packed sequences ----------------
+    @staticmethod
+    def _axis_tables(rope: AxisRope | None, head_dim: int, x: torch.Tensor):
+        """cos, sin [T, 1, head_dim / 2]; pairs without an axis do not turn."""
+        half = head_dim // 2
+        angles = torch.zeros(x.shape[0], half, dtype=torch.float64, device=x.device)
+        if rope is not None:
+            if rope.positions.shape[0] != x.shape[0] or sum(rope.pairs) > half:
+                raise ValueError("the rotation does not fit q's tokens and head_dim")
+            n = sum(rope.pairs)
+            angles[:, :n] = rope.positions.double()[:, rope.axis_of_pairs()] * rope.freqs.double()
+        dtype = torch.promote_types(x.dtype, torch.float32)
+        return angles.cos().to(dtype)[:, None], angles.sin().to(dtype)[:, None]
+
+    @staticmethod
+    def _turn(x, cos, sin, interleaved: bool):
+        a, b = (x[..., 0::2], x[..., 1::2]) if interleaved else x.chunk(2, -1)
+        y = a * cos - b * sin, a * sin + b * cos
+        return torch.stack(y, -1).flatten(-2) if interleaved else torch.cat(y, -1)
+
+    def rope_axes(self, q, k, rope: AxisRope, inverse: bool = False):
+        """Rotate every head of ``q`` and ``k`` (``k`` may be None); ``inverse`` turns gradients back."""
+        cos, sin = self._axis_tables(rope, q.shape[-1], q)
+        sin = -sin if inverse else sin
+        return tuple(None if x is None else self._turn(x.to(cos.dtype), cos, sin, rope.interleaved).to(x.dtype)
+                     for x in (q, k))
+
+    def qk_norm_rope(self, q, k, q_weight, k_weight, rope: AxisRope | None = None, eps=1e-6):
+        """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``), then the rotation."""
+        cos, sin = self._axis_tables(rope, q.shape[-1], q)
+        out = []
+        for x, w in ((q, q_weight), (k, k_weight)):
+            xf = x.to(cos.dtype)
+            n = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.to(cos.dtype)
+            out.append(self._turn(n, cos, sin, rope is None or rope.interleaved).to(x.dtype))
+        return tuple(out)
+
+    def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6):
+        """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32."""
+        cos, sin = self._axis_tables(rope, q.shape[-1], q)
+        grads, weights = [], []
+        for x, w, dy in ((q, q_weight, dq), (k, k_weight, dk)):
+            xf = x.to(cos.dtype)
+            r = torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
+            n = xf * r
+            g = self._turn(dy.to(cos.dtype), cos, -sin, rope is None or rope.interleaved)
+            gw = g * w.to(cos.dtype)
+            grads.append((r * (gw - n * (gw * n).mean(-1, keepdim=True))).to(x.dtype))
+            weights.append((g * n).sum((0, 1)))
+        return grads[0], grads[1], weights[0], weights[1]
+
+    def packed_plan(self, q_lens, k_lens=None, *, heads, kv_heads, head_dim, causal=False) -> PackedPlan:
+        return PackedPlan.lengths(q_lens, k_lens, heads=heads, kv_heads=kv_heads, head_dim=head_dim, causal=causal)
+
+    @staticmethod
+    def _check_packed(q, k, v, plan: PackedPlan) -> None:
+        want_q = (plan.q_tokens, plan.heads, plan.head_dim)
+        want_k = (plan.k_tokens, plan.kv_heads, plan.head_dim)
+        if tuple(q.shape) != want_q or tuple(k.shape) != want_k or tuple(v.shape) != want_k:
+            raise ValueError(f"q, k, v must be {want_q}, {want_k}, {want_k} as planned, got "
+                             f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+
+    @staticmethod
+    def _packed_sequences(plan: PackedPlan, device):
+        """(query rows, key rows, hidden mask or None) of every sequence."""
+        q0 = k0 = 0
+        for nq, nk in zip(plan.q_lens, plan.k_lens):
+            hidden = None
+            if plan.causal:
+                i, j = torch.arange(nq, device=device), torch.arange(nk, device=device)
+                hidden = j[None, :] - nk > i[:, None] - nq
+            yield slice(q0, q0 + nq), slice(k0, k0 + nk), hidden
+            q0, k0 = q0 + nq, k0 + nk
+
+    def attention_packed_fwd(self, q, k, v, plan: PackedPlan, scale=None):
+        """Attention of each sequence of a packed batch with itself -> (o, lse [heads, tokens] fp32).
+
+        ``q [tokens, heads, D]``, ``k, v [tokens, kv_heads, D]``; query head ``h``
+        reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to
+        ``1 / sqrt(D)``.  A query that sees no key gives o = 0 and lse = -inf.
+        Values of keys that a query does not see have no weight, but as in any
+        product 0 * NaN is NaN: keys and values within one sequence must be finite.
+        What lies outside a sequence (other sequences of the batch) is never read into it.
+        """
+        self._check_packed(q, k, v, plan)
+        scale = plan.head_dim ** -0.5 if scale is None else scale
+        group = plan.heads // plan.kv_heads
+        dtype = torch.promote_types(q.dtype, torch.float32)
+        o = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.full((plan.heads, q.shape[0]), -math.inf, dtype=dtype, device=q.device)
+        for rq, rk, hidden in self._packed_sequences(plan, q.device):
+            if rq.start == rq.stop or rk.start == rk.stop:
+                continue
+            qs = q[rq].to(dtype).transpose(0, 1)
+            ks, vs = (x[rk].to(dtype).transpose(0, 1).repeat_interleave(group, 0) for x in (k, v))
+            s = scale * (qs @ ks.transpose(1, 2))
+            if hidden is not None:
+                s = s.masked_fill(hidden, -math.inf)
+            row = torch.logsumexp(s, -1)
+            p = torch.exp(s - row.masked_fill(row == -math.inf, 0.0)[..., None])
+            o[rq] = (p @ vs).transpose(0, 1).to(o.dtype)
+            lse[:, rq] = row
+        return o, lse
+
+    def attention_packed_bwd(self, q, k, v, o, lse, do, plan: PackedPlan, scale=None, out=None):
+        """Gradients ``(dq, dk, dv)``; ``out``: three tensors (views are fine) to write them into."""
+        self._check_packed(q, k, v, plan)
+        scale = plan.head_dim ** -0.5 if scale is None else scale
+        group = plan.heads // plan.kv_heads
+        dtype = torch.promote_types(q.dtype, torch.float32)
+        grads = out if out is not None else tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                                                  for x in (q, k, v))
+        for g in grads:
+            g.zero_()
+        for rq, rk, hidden in self._packed_sequences(plan, q.device):
+            if rq.start == rq.stop or rk.start == rk.stop:
+                continue
+            qs, dos, os_ = (x[rq].to(dtype).transpose(0, 1) for x in (q, do, o))
+            ks, vs = (x[rk].to(dtype).transpose(0, 1).repeat_interleave(group, 0) for x in (k, v))
+            s = scale * (qs @ ks.transpose(1, 2))
+            row = lse[:, rq].to(dtype)
+            p = torch.exp(s - row.masked_fill(row == -math.inf, math.inf)[..., None])
+            if hidden is not None:
+                p = p.masked_fill(hidden, 0.0)
+            ds = scale * p * (dos @ vs.transpose(1, 2) - (dos * os_).sum(-1, keepdim=True))
+
+            def per_key_head(x):
+                return x.unflatten(0, (plan.kv_heads, group)).sum(1).transpose(0, 1)
+
+            grads[0][rq] = (ds @ ks).transpose(0, 1).to(grads[0].dtype)
+            grads[1][rk] = per_key_head(ds.transpose(1, 2) @ qs).to(grads[1].dtype)
+            grads[2][rk] = per_key_head(p.transpose(1, 2) @ dos).to(grads[2].dtype)
+        return tuple(grads)
 
     # ---------------- small projections ----------------
     def adaln_project(self, temb, w, b):

@@ -18,6 +18,10 @@ SOURCES = [
     "csrc/elementwise/elementwise.cu",
     "csrc/attn/attention_fwd.cu",
     "csrc/attn/attention_bwd.cu",
+    "csrc/attn/packed_fwd.cu",
+    "csrc/attn/packed_bwd.cu",
+    "csrc/attn/packed_host.cu",
+    "csrc/rope/qk_rope.cu",
     "csrc/noalloc/dmd_loss_noalloc.cu",
     "csrc/comm/p2p.cu",
     "csrc/staging/pinned_pool.cpp",
@@ -55,6 +59,10 @@ CHECKED_SOURCES = [
     "csrc/checked/checked_elementwise.cu",
     "csrc/checked/checked_attention_fwd.cu",
     "csrc/checked/checked_attention_bwd.cu",
+    "csrc/checked/checked_packed_fwd.cu",
+    "csrc/checked/checked_packed_bwd.cu",
+    "csrc/checked/checked_packed_host.cu",
+    "csrc/checked/checked_qk_rope.cu",
     "csrc/checked/checked_p2p.cu",
     "csrc/checked/checked_pinned_pool.cpp",
 ]
