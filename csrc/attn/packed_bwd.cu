@@ -51,80 +51,6 @@ struct Bwd {
   static_assert(kSmem <= 232448, "shared memory");
 };
 
-__device__ __forceinline__ PackedItem load_item(const PackedItem* p) {
-  PackedItem it;
-  const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
-  it.q0 = a.x, it.nq = a.y, it.k0 = a.z, it.nk = a.w, it.diag = b.x, it.head = b.y, it.slot = b.z, it.pad = b.w;
-  return it;
-}
-
-// A ring of tiles.  A tile whose last rows must be zeroed arrives on tail[slot];
-// the cleaning warp then makes the arrival on full[slot].
-template <int SLOTS>
-struct Ring {
-  uint64_t *full, *empty, *tail;
-  uint8_t* base;
-  static constexpr int kBarriers = 3 * SLOTS;
-  __device__ __forceinline__ void place(uint64_t* bars, uint8_t* tiles) {
-    full = bars, empty = bars + SLOTS, tail = bars + 2 * SLOTS, base = tiles;
-  }
-  __device__ __forceinline__ void init() const {
-    for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-      mbar_init(&tail[s], 1);
-    }
-  }
-  __device__ __forceinline__ static int slot(int n) { return n % SLOTS; }
-  __device__ __forceinline__ bool wait_full(int n, uint64_t limit, volatile int* abort) const {
-    return mbar_wait(&full[n % SLOTS], static_cast<uint32_t>(n / SLOTS) & 1u, limit, abort);
-  }
-};
-
-// The loader's side of a ring.
-template <int SLOTS>
-struct Feed {
-  int n = 0;
-  uint32_t tail_slots = 0, tail_parity = 0;
-  // Waits for the next slot and arms its barrier; null if the wait gave up.
-  __device__ __forceinline__ uint64_t* next(const Ring<SLOTS>& r, bool tail, uint32_t bytes, uint64_t limit,
-                                            volatile int* abort, int& slot) {
-    slot = n % SLOTS;
-    if (!mbar_wait(&r.empty[slot], (static_cast<uint32_t>(n / SLOTS) & 1u) ^ 1u, limit, abort)) return nullptr;
-    uint64_t* full = tail ? &r.tail[slot] : &r.full[slot];
-    tail_slots = (tail_slots & ~(1u << slot)) | (tail ? 1u << slot : 0u);
-    if (tail) tail_parity ^= 1u << slot;
-    mbar_arrive_expect_tx(full, bytes);
-    ++n;
-    return full;
-  }
-  // Never leave a TMA write in flight into this CTA's shared memory.
-  __device__ __forceinline__ void drain(const Ring<SLOTS>& r, uint64_t limit) const {
-    volatile int never = 0;
-    for (int s = 0; s < min(n, SLOTS); ++s) {
-      const int last = (n - 1 - s) / SLOTS * SLOTS + s;
-      if (tail_slots >> s & 1u)
-        mbar_wait(&r.tail[s], (tail_parity >> s & 1u) ^ 1u, limit, &never);
-      else
-        mbar_wait(&r.full[s], static_cast<uint32_t>(last / SLOTS) & 1u, limit, &never);
-    }
-  }
-};
-
-// One tail tile of a ring (all lanes of the cleaning warp).
-template <int CHUNKS, int TILE, int SLOTS>
-__device__ __forceinline__ bool clean_tile(const Ring<SLOTS>& r, int n, int first, uint32_t& parity, uint64_t limit,
-                                           volatile int* abort) {
-  const int slot = n % SLOTS;
-  if (!__all_sync(0xffffffffu, mbar_wait(&r.tail[slot], parity >> slot & 1u, limit, abort))) return false;
-  parity ^= 1u << slot;
-  zero_tile_rows<CHUNKS>(r.base + slot * TILE, first);
-  fence_async_smem();
-  __syncwarp();
-  if (lane_id() == 0) mbar_arrive(&r.full[slot]);
-  return true;
-}
-
 // S-shaped product of two K-major tiles: D[tmem] = A B^T over D columns.
 template <int D>
 __device__ __forceinline__ void issue_scores(uint32_t d_tmem, const uint8_t* a, const uint8_t* b) {

@@ -8,22 +8,27 @@
 //
 // Persistent: each block walks its slice of a work list that the host has
 // balanced over the SMs; barriers and TMEM are set up once and the ring of K/V
-// tiles runs on across items.  384 threads:
-//   warp 0      TMA: the item's one or two query tiles, then K_0 V_0 K_1 V_1 ...
-//   warp 1      tcgen05.mma issuer (one thread), S_t = Q_t K_j^T into TMEM and
-//               O_t += P_t V_j with P_t read from TMEM, in the order
-//               S_0 S_1 | PV_0 S_0' PV_1 S_1' | ..., so that the tensor core
-//               works on one query tile during the other's softmax
+// tiles runs on across items.  Two softmax warpgroups t = 0, 1 run side by side,
+// each with its own running m, l and TMEM accumulator O_t.  An item of two query
+// tiles gives one to each (shared key tiles); an item of one query tile gives
+// the even key tiles to one and the odd ones to the other, and the two
+// accumulators are joined in the epilogue.  384 threads:
+//   warp 0      TMA: the query tiles, then K_0 V_0 K_1 V_1 ... through the ring
+//   warp 1      issues S = Q K^T into TMEM (one thread)
+//   warp 3      issues O_t += P_t V with P_t read from TMEM (one thread); issuing
+//               a product takes about 500 cycles of scalar work, so one thread
+//               for both would set the pace
 //   warp 2      zeroes the rows of the last V tile that lie past its sequence:
 //               they belong to the next sequence and 0 * NaN would leak
-//   warps 4..7  softmax of query tile 0, warps 8..11 of tile 1, one row a thread;
-//               P as packed bf16 pairs over the consumed S columns
-// P is rounded to bf16 (the MMA's operand type, as q, k and v are); l is summed
-// from the unrounded fp32 values, O accumulates in fp32.
-// Few rows over many keys (single new tokens): the host splits the key axis
-// over blocks; parts are normalised on their own, kept in fp32 with their
-// log-sum-exp, and joined by packed_join_kernel in a fixed order.
-// Every wait is bounded (ptx.cuh); every TMA load targets one CTA only.
+//   warps 4..7 and 8..11  softmax, one query row a thread
+// TMEM columns: S [0,128)  P_0 [128,192)  P_1 [192,256)  O_0 [256,384)  O_1 [384,512).
+// What sets the pace is the exponentials (16 a cycle and SM: 2,048 cycles for two
+// 128 x 128 tiles, as many as their four products take), if nothing waits.  So P
+// has columns of its own and S is shared by both warpgroups: S_t is taken into
+// registers in about 100 cycles, then the next S (the other warpgroup's) is
+// issued at once and is ready before that warpgroup has finished its current
+// exponentials.  With P over the consumed S columns (S_0 S_1 in 256 columns) the
+// next S_t had to wait for PV_t, and a step was the chain softmax -> PV -> S.
 #include "../common/ptx.cuh"
 #include "packed.h"
 #include "tile.cuh"
@@ -45,62 +50,69 @@ template <int D>
 struct Fwd {
   static constexpr int kChunks = D / 64;
   static constexpr int kTile = kChunks * kChunkBytes;
-  static constexpr int kSlots = D == 128 ? 5 : 10;   // ring of K/V tiles: all that fits beside two Q tiles
-  static constexpr int kSmem = 1024 + (2 + kSlots) * kTile + 512;
+  // Rings of K and V tiles: all that fits beside two Q tiles.  A K tile is free
+  // after its scores, a V tile a step later, after its values.
+  static constexpr int kK = D == 128 ? 2 : 5, kV = D == 128 ? 3 : 5;
+  static constexpr int kSmem = (2 + kK + kV) * kTile + 2048 + 512;   // tiles, exchanged m and l, barriers
   static_assert(kSmem <= 232448, "shared memory");
 };
 
 struct Bars {
-  uint64_t *q_full, *q_empty, *slot_full, *slot_empty, *s_full, *p_full, *o_done, *drain;
-  uint64_t* tail_full;   // per ring slot: a V tile with rows past its sequence arrived (before slot_full, see clean_warp)
+  uint64_t *q_full, *q_empty;
+  uint64_t *s_full;      // [t] S_t is in TMEM
+  uint64_t *s_taken;     // S is in its warpgroup's registers, the columns are free
+  uint64_t *p_full;      // [t] P_t is in TMEM
+  uint64_t *pv_done;     // [t] PV_t is complete
+  uint64_t *drain;       // [2] the issuers' last products are complete
 };
 
+// What an item asks of the two warpgroups.
 struct TileWork {
-  int n[2];      // key tiles of each query tile
-  int rows[2];   // live rows of each query tile
-  int most, tail;   // key tiles loaded; live rows of the last one if it is cut short, else 0
+  int n0, n1;      // key tiles of each
+  int most, tail;  // key tiles loaded; live rows of the last one if it is cut short, else 0
+  bool solo;       // one query tile: key tile 2 j + t is step j of warpgroup t, else key tile j
+  __device__ __forceinline__ int n(int t) const { return t == 0 ? n0 : n1; }
+  __device__ __forceinline__ int key_tile(int t, int j) const { return solo ? 2 * j + t : j; }
 };
 
-__device__ __forceinline__ TileWork tile_work(const PackedItem& it, int bt, int G) {
+__device__ __forceinline__ int tiles_seen(const PackedItem& it, int first, int tokens) {
+  const int seen = tokens > 0 ? min(it.nk, max(0, first + tokens + it.diag)) : 0;
+  return (seen + 127) >> 7;
+}
+
+__device__ __forceinline__ TileWork tile_work(const PackedItem& it, int bt) {
   TileWork w;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int tokens = max(0, min(bt, it.nq - t * bt));
-    const int seen = tokens > 0 ? min(it.nk, max(0, t * bt + tokens + it.diag)) : 0;
-    w.n[t] = (seen + 127) >> 7;
-    w.rows[t] = tokens * G;
+  w.solo = it.nq <= bt;
+  w.n0 = tiles_seen(it, 0, min(bt, it.nq));
+  w.n1 = w.solo ? 0 : tiles_seen(it, bt, it.nq - bt);
+  w.most = max(w.n0, w.n1);
+  if (w.solo) {
+    w.n1 = w.n0 >> 1;
+    w.n0 -= w.n1;
   }
-  w.most = max(w.n[0], w.n[1]);
   const int left = it.nk - (w.most - 1) * 128;
   w.tail = (w.most > 0 && left < 128) ? left : 0;
   return w;
 }
 
-__device__ __forceinline__ PackedItem load_item(const PackedItem* p) {
-  PackedItem it;
-  const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
-  it.q0 = a.x, it.nq = a.y, it.k0 = a.z, it.nk = a.w, it.diag = b.x, it.head = b.y, it.slot = b.z, it.pad = b.w;
-  return it;
-}
-
 template <int D>
 __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                                          const PackedFwdParams& p, uint8_t* sQ, uint8_t* ring, const Bars& b,
-                                          volatile int* abort_flag) {
+                                          const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kK>& rk,
+                                          const Ring<Fwd<D>::kV>& rv, const Bars& b, volatile int* abort_flag) {
   using C = Fwd<D>;
   const uint64_t limit = p.status.limit_ns;
   const uint32_t q_bytes = static_cast<uint32_t>(p.bt * p.G) * 128u * C::kChunks;
-  int n = 0, slot = 0, filled = 0;      // loads so far, their ring slot
-  uint32_t phase = 0, tail_slots = 0, tail_parity = 0;   // bit per slot: its last load is a tail; parity of its next tail
+  Feed<C::kK> fk;
+  Feed<C::kV> fv;
   int q_used[2] = {0, 0};
   bool ok = true;
   const int end = p.begin[blockIdx.x + 1];
   for (int i = p.begin[blockIdx.x]; i < end && ok; ++i) {
     const PackedItem it = load_item(p.items + i);
-    const TileWork w = tile_work(it, p.bt, p.G);
+    const TileWork w = tile_work(it, p.bt);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (w.n[t] == 0 || !ok) continue;
+      if (w.n(t) == 0 || (w.solo && t == 1) || !ok) continue;
       if (!mbar_wait(&b.q_empty[t], (q_used[t] & 1) ^ 1u, limit, abort_flag)) {
         ok = false;
         break;
@@ -111,164 +123,151 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorM
       for (int c = 0; c < C::kChunks; ++c)
         tma_load_4d(sQ + t * C::kTile + c * kChunkBytes, &tq, &b.q_full[t], c * 64, 0, it.head, it.q0 + t * p.bt);
     }
-    for (int m = 0; m < 2 * w.most && ok; ++m) {
-      if (!mbar_wait(&b.slot_empty[slot], phase ^ 1u, limit, abort_flag)) {
-        ok = false;
-        break;
-      }
-      const CUtensorMap* map = (m & 1) ? &tv : &tk;
-      const bool tail = w.tail != 0 && m == 2 * w.most - 1;
-      uint64_t* full = tail ? &b.tail_full[slot] : &b.slot_full[slot];
-      tail_slots = (tail_slots & ~(1u << slot)) | (tail ? 1u << slot : 0u);
-      if (tail) tail_parity ^= 1u << slot;
-      mbar_arrive_expect_tx(full, C::kTile);
+    for (int kt = 0; kt < w.most && ok; ++kt) {
+      int slot;
+      uint64_t* full = fk.next(rk, false, C::kTile, limit, abort_flag, slot);
+      ok = full != nullptr;
+      if (!ok) break;
 #pragma unroll
       for (int c = 0; c < C::kChunks; ++c)
-        tma_load_3d(ring + slot * C::kTile + c * kChunkBytes, map, full, c * 64, it.head, it.k0 + (m >> 1) * 128);
-      ++n;
-      filled = min(C::kSlots, n);
-      if (++slot == C::kSlots) {
-        slot = 0;
-        phase ^= 1u;
-      }
+        tma_load_3d(rk.base + slot * C::kTile + c * kChunkBytes, &tk, full, c * 64, it.head, it.k0 + kt * 128);
+      full = fv.next(rv, w.tail != 0 && kt + 1 == w.most, C::kTile, limit, abort_flag, slot);
+      ok = full != nullptr;
+      if (!ok) break;
+#pragma unroll
+      for (int c = 0; c < C::kChunks; ++c)
+        tma_load_3d(rv.base + slot * C::kTile + c * kChunkBytes, &tv, full, c * 64, it.head, it.k0 + kt * 128);
     }
   }
   if (!ok) {
-    report_status(p.status, kStatusTimeoutEmpty, n);
+    report_status(p.status, kStatusTimeoutEmpty, fk.n);
     *abort_flag = 1;
   }
-  // Never leave a TMA write in flight into this CTA's shared memory.
+  fk.drain(rk, limit);
+  fv.drain(rv, limit);
   volatile int never = 0;
   for (int t = 0; t < 2; ++t)
     if (q_used[t] > 0) mbar_wait(&b.q_full[t], (q_used[t] - 1) & 1, limit, &never);
-  for (int s = 0; s < filled; ++s) {
-    const int last = (n - 1 - s) / C::kSlots * C::kSlots + s;   // the latest load into slot s
-    if (tail_slots >> s & 1u)
-      mbar_wait(&b.tail_full[s], (tail_parity >> s & 1u) ^ 1u, limit, &never);
-    else
-      mbar_wait(&b.slot_full[s], (last / C::kSlots) & 1, limit, &never);
-  }
 }
 
-template <int D>
-__device__ __forceinline__ void mma_warp(const PackedFwdParams& p, uint8_t* sQ, uint8_t* ring, const Bars& b,
-                                         volatile int* abort_flag, uint32_t tmem) {
-  using C = Fwd<D>;
-  constexpr uint32_t kIdescS = umma_idesc_bf16(128, 128, false, false);
-  constexpr uint32_t kIdescPV = umma_idesc_bf16(128, D, false, true);
-  const uint64_t limit = p.status.limit_ns;
-  int base = 0;            // ring index of the item's K_0
-  int q_used[2] = {0, 0}, steps[2] = {0, 0};
-  bool ok = true, any = false;
-  auto wait_slot = [&](int n) {
-    return mbar_wait(&b.slot_full[n % C::kSlots], static_cast<uint32_t>(n / C::kSlots) & 1u, limit, abort_flag);
-  };
-  auto issue_s = [&](int t, int j) {
-    const uint32_t q_base = smem_u32(sQ + t * C::kTile);
-    const uint32_t k_base = smem_u32(ring + ((base + 2 * j) % C::kSlots) * C::kTile);
-#pragma unroll
-    for (int ds = 0; ds < D / 16; ++ds) {
-      const uint32_t off = (ds >> 2) * kChunkBytes + (ds & 3) * 32;
-      umma_f16_ss(tmem + t * 128, umma_smem_desc(q_base + off, 16, 1024), umma_smem_desc(k_base + off, 16, 1024),
-                  kIdescS, ds > 0 ? 1u : 0u);
-    }
-    umma_commit(&b.s_full[t]);
-    any = true;
-  };
-  auto issue_pv = [&](int t, int j) {
-    const uint32_t v_base = smem_u32(ring + ((base + 2 * j + 1) % C::kSlots) * C::kTile);
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks)
-      umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, umma_smem_desc(v_base + ks * 2048, kChunkBytes, 1024),
-                  kIdescPV, (j > 0 || ks > 0) ? 1u : 0u);
-  };
-  const int end = p.begin[blockIdx.x + 1];
-  for (int i = p.begin[blockIdx.x]; i < end && ok; ++i) {
-    const PackedItem it = load_item(p.items + i);
-    const TileWork w = tile_work(it, p.bt, p.G);
-    if (w.most == 0) continue;
-    ok = wait_slot(base);
-    for (int t = 0; t < 2 && ok; ++t) {
-      if (w.n[t] == 0) continue;
-      ok = mbar_wait(&b.q_full[t], q_used[t] & 1, limit, abort_flag);
-      if (!ok) break;
-      ++q_used[t];
-      tc_fence_after();
-      issue_s(t, 0);
-      if (w.n[t] == 1) umma_commit(&b.q_empty[t]);
-    }
-    if (ok) umma_commit(&b.slot_empty[base % C::kSlots]);
-    for (int j = 0; j < w.most && ok; ++j) {
-      const int last_pv = j < w.n[1] ? 1 : 0, last_s = j + 1 < w.n[1] ? 1 : 0;
-      bool have_v = false, have_k = false;
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (j >= w.n[t]) continue;
-        ok = mbar_wait(&b.p_full[t], steps[t] & 1, limit, abort_flag) && (have_v || wait_slot(base + 2 * j + 1));
-        if (!ok) break;
-        have_v = true;
-        ++steps[t];
-        tc_fence_after();
-        issue_pv(t, j);
-        if (j + 1 == w.n[t]) umma_commit(&b.o_done[t]);
-        if (t == last_pv) umma_commit(&b.slot_empty[(base + 2 * j + 1) % C::kSlots]);
-        if (j + 1 < w.n[t]) {
-          if (!have_k) {
-            ok = wait_slot(base + 2 * j + 2);
-            have_k = true;
-            if (!ok) break;
-            tc_fence_after();
-          }
-          issue_s(t, j + 1);
-          if (j + 2 == w.n[t]) umma_commit(&b.q_empty[t]);
-          if (t == last_s) umma_commit(&b.slot_empty[(base + 2 * j + 2) % C::kSlots]);
-        }
-      }
-    }
-    base += 2 * w.most;
-  }
+// Ends an issuer: no product of this thread may still read shared memory or TMEM.
+__device__ __forceinline__ void finish_issuer(uint64_t* drain, bool any, bool ok, int where, const KernelStatus& st,
+                                              volatile int* abort_flag) {
   if (!ok) {
-    report_status(p.status, kStatusTimeoutFull, base);
+    report_status(st, kStatusTimeoutFull, where);
     *abort_flag = 1;
   }
   if (any) {
-    umma_commit(b.drain);
+    umma_commit(drain);
     volatile int never = 0;
-    mbar_wait(b.drain, 0, limit, &never);
+    mbar_wait(drain, 0, st.limit_ns, &never);
   }
 }
 
-// Zeroes the rows past the sequence in the last V tile of each item that has
-// such rows.  That tile's load arrives on tail_full[slot]; this warp then makes
-// the arrival that the MMA issuer waits for on slot_full[slot].  A barrier per
-// slot: a slot is loaded again only after its tile was consumed, so this warp
-// can never miss a phase.
+// All scores, in the order (key tile, warpgroup).
 template <int D>
-__device__ __forceinline__ void clean_warp(const PackedFwdParams& p, uint8_t* ring, const Bars& b,
+__device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kK>& rk, const Bars& b,
+                                           volatile int* abort_flag, uint32_t tmem) {
+  using C = Fwd<D>;
+  constexpr uint32_t kIdesc = umma_idesc_bf16(128, 128, false, false);
+  const uint64_t limit = p.status.limit_ns;
+  const uint64_t q_desc = umma_smem_desc(smem_u32(sQ), 16, 1024), k_desc = umma_smem_desc(smem_u32(rk.base), 16, 1024);
+  Cursor<C::kK> k;
+  uint32_t q_used0 = 0, q_used1 = 0, issued = 0;
+  bool ok = true;
+  const int end = p.begin[blockIdx.x + 1];
+  for (int i = p.begin[blockIdx.x]; i < end && ok; ++i) {
+    const TileWork w = tile_work(load_item(p.items + i), p.bt);
+    for (int kt = 0; kt < w.most && ok; ++kt, k.next()) {
+      ok = mbar_wait(&rk.full[k.slot], k.phase, limit, abort_flag);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || (w.solo ? t != (kt & 1) : kt >= w.n(t))) continue;
+        const int tile = w.solo ? 0 : t;
+        if (kt == 0) {
+          uint32_t& used = tile == 0 ? q_used0 : q_used1;
+          ok = mbar_wait(&b.q_full[tile], used & 1u, limit, abort_flag);
+          ++used;
+        }
+        // The last S is taken; with it the one before this warpgroup's P went into its own columns.
+        ok = ok && (issued == 0 || mbar_wait(b.s_taken, (issued - 1) & 1u, limit, abort_flag));
+        if (!ok) continue;
+        ++issued;
+        tc_fence_after();
+        const uint64_t qd = q_desc + static_cast<uint64_t>(tile * (C::kTile >> 4));
+        const uint64_t kd = k_desc + static_cast<uint64_t>(k.slot * (C::kTile >> 4));
+#pragma unroll
+        for (int ds = 0; ds < D / 16; ++ds) {
+          constexpr int kChunk16 = kChunkBytes >> 4;
+          const uint64_t off = (ds >> 2) * kChunk16 + (ds & 3) * 2;
+          umma_f16_ss(tmem, qd + off, kd + off, kIdesc, ds > 0 ? 1u : 0u);
+        }
+        umma_commit(&b.s_full[t]);
+        if (kt + 1 == (w.solo ? w.most : w.n(t))) umma_commit(&b.q_empty[tile]);
+      }
+      if (ok) umma_commit(&rk.empty[k.slot]);
+    }
+  }
+  finish_issuer(&b.drain[0], issued > 0, ok, static_cast<int>(issued), p.status, abort_flag);
+}
+
+// All products with V, in the same order.
+template <int D>
+__device__ __forceinline__ void value_warp(const PackedFwdParams& p, const Ring<Fwd<D>::kV>& rv, const Bars& b,
+                                           volatile int* abort_flag, uint32_t tmem) {
+  using C = Fwd<D>;
+  constexpr uint32_t kIdesc = umma_idesc_bf16(128, D, false, true);
+  const uint64_t limit = p.status.limit_ns;
+  const uint64_t v_desc = umma_smem_desc(smem_u32(rv.base), kChunkBytes, 1024);
+  Cursor<C::kV> v;
+  uint32_t steps0 = 0, steps1 = 0;
+  bool ok = true;
+  const int end = p.begin[blockIdx.x + 1];
+  for (int i = p.begin[blockIdx.x]; i < end && ok; ++i) {
+    const TileWork w = tile_work(load_item(p.items + i), p.bt);
+    for (int kt = 0; kt < w.most && ok; ++kt, v.next()) {
+      ok = mbar_wait(&rv.full[v.slot], v.phase, limit, abort_flag);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || (w.solo ? t != (kt & 1) : kt >= w.n(t))) continue;
+        uint32_t& steps = t == 0 ? steps0 : steps1;
+        ok = mbar_wait(&b.p_full[t], steps & 1u, limit, abort_flag);
+        if (!ok) continue;
+        ++steps;
+        tc_fence_after();
+        const uint64_t vd = v_desc + static_cast<uint64_t>(v.slot * (C::kTile >> 4));
+        const uint32_t more = kt > (w.solo ? t : 0) ? 1u : 0u;      // O_t holds earlier tiles
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+          umma_f16_ts(tmem + 256 + t * 128, tmem + 128 + t * 64 + ks * 8, vd + static_cast<uint64_t>(ks * 128), kIdesc,
+                      ks > 0 ? 1u : more);
+        umma_commit(&b.pv_done[t]);
+      }
+      if (ok) umma_commit(&rv.empty[v.slot]);
+    }
+  }
+  finish_issuer(&b.drain[1], steps0 + steps1 > 0, ok, static_cast<int>(steps0 + steps1), p.status, abort_flag);
+}
+
+// Zeroes the rows past the sequence in the last V tile of each item that has such rows.
+template <int D>
+__device__ __forceinline__ void clean_warp(const PackedFwdParams& p, const Ring<Fwd<D>::kV>& rv,
                                            volatile int* abort_flag) {
   using C = Fwd<D>;
   int base = 0;
   uint32_t parity = 0;
   const int end = p.begin[blockIdx.x + 1];
   for (int i = p.begin[blockIdx.x]; i < end; ++i) {
-    const PackedItem it = load_item(p.items + i);
-    const TileWork w = tile_work(it, p.bt, p.G);
-    if (w.tail != 0) {
-      const int slot = (base + 2 * w.most - 1) % C::kSlots;
-      const bool ok = mbar_wait(&b.tail_full[slot], parity >> slot & 1u, p.status.limit_ns, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) {
-        if (lane_id() == 0) {
-          report_status(p.status, kStatusTimeoutFull, i);
-          *abort_flag = 1;
-        }
-        return;
+    const TileWork w = tile_work(load_item(p.items + i), p.bt);
+    if (w.tail != 0 &&
+        !clean_tile<C::kChunks, C::kTile>(rv, base + w.most - 1, w.tail, parity, p.status.limit_ns, abort_flag)) {
+      if (lane_id() == 0) {
+        report_status(p.status, kStatusTimeoutFull, i);
+        *abort_flag = 1;
       }
-      parity ^= 1u << slot;
-      zero_tile_rows<C::kChunks>(ring + slot * C::kTile, w.tail);
-      fence_async_smem();
-      __syncwarp();
-      if (lane_id() == 0) mbar_arrive(&b.slot_full[slot]);
+      return;
     }
-    base += 2 * w.most;
+    base += w.most;
   }
 }
 
@@ -286,13 +285,12 @@ __device__ __forceinline__ float row_max(const uint32_t (&r)[4][32]) {
   return fmaxf(fmax3(m[0], m[1], m[2]), fmax3(fmax3(m[3], m[4], m[5]), m[6], m[7]));
 }
 
-// P = 2^(s * scale - m) as packed bf16 pairs over the first 64 S columns; returns the fp32 row sum.
-__device__ __forceinline__ float row_exp(uint32_t tS, const uint32_t (&r)[4][32], float scale, float m) {
+// P = 2^(s * scale - m) as packed bf16 pairs, in place of the row's first 64 registers; returns the fp32 row sum.
+__device__ __forceinline__ float row_exp(uint32_t (&r)[4][32], float scale, float m) {
   const uint64_t scale2 = pack2(scale, scale), negm2 = pack2(-m, -m);
   uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t packed[16];
+  for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float a, b;
@@ -300,10 +298,8 @@ __device__ __forceinline__ float row_exp(uint32_t tS, const uint32_t (&r)[4][32]
       a = ex2(a);
       b = ex2(b);
       acc[i & 3] = add2(acc[i & 3], pack2(a, b));
-      packed[i] = pack_bf16x2(a, b);
+      r[c >> 1][(c & 1) * 16 + i] = pack_bf16x2(a, b);
     }
-    tmem_st16(tS + c * 16, packed);
-  }
   float a, b;
   unpack2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), a, b);
   return a + b;
@@ -311,23 +307,24 @@ __device__ __forceinline__ float row_exp(uint32_t tS, const uint32_t (&r)[4][32]
 
 template <int D>
 __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Bars& b, volatile int* abort_flag,
-                                              uint32_t tmem, int t) {
+                                              float2* exchange, uint32_t tmem, int t) {
   const uint64_t limit = p.status.limit_ns;
   const int row = (warp_id() & 3) * 32 + lane_id();
   const uint32_t lane_off = static_cast<uint32_t>((warp_id() & 3) * 32) << 16;
-  const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
+  const uint32_t tS = tmem + lane_off, tP = tmem + 128 + t * 64 + lane_off, tO = tmem + 256 + lane_off;
   const int tok = row / p.G, g = row - tok * p.G;   // token of the tile and head of the group of this row
-  int steps = 0, done = 0;
+  int steps = 0;          // this warpgroup's key tiles so far
   bool ok = true;
   const int end = p.begin[blockIdx.x + 1];
   for (int i = p.begin[blockIdx.x]; i < end; ++i) {
     const PackedItem it = load_item(p.items + i);
-    const TileWork w = tile_work(it, p.bt, p.G);
-    const int n_kv = w.n[t];
-    if (w.rows[t] == 0) continue;
-    const bool live = row < w.rows[t];
+    const TileWork w = tile_work(it, p.bt);
+    const int first = w.solo ? 0 : t * p.bt, n_kv = w.n(t);
+    const bool both = w.solo && w.n1 > 0;      // one query tile, both warpgroups on it
+    if (w.solo ? t == 1 && !both : it.nq <= first) continue;
+    const bool live = row < min(p.bt, it.nq - first) * p.G;
     // Keys that this row sees; rows that are not stored see every key of the item.
-    const int seen = live ? min(it.nk, max(0, t * p.bt + tok + it.diag + 1)) : it.nk;
+    const int seen = live ? min(it.nk, max(0, first + tok + it.diag + 1)) : it.nk;
     float m = -INFINITY, l = 0.f;
     for (int j = 0; j < n_kv; ++j, ++steps) {
       // Warp-uniform outcome: tcgen05.ld/st below are warp-collective.
@@ -338,7 +335,9 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
       tmem_ld_wait();
-      const int valid = seen - j * 128;
+      tc_fence_before();
+      mbar_arrive(b.s_taken);
+      const int valid = seen - w.key_tile(t, j) * 128;
       if (__any_sync(0xffffffffu, valid < 128)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -354,17 +353,24 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
         l *= alpha;
         m = m_new;
       }
-      l += row_exp(tS, r, p.scale_log2, m == -INFINITY ? 0.f : m);
-      // S_t(j) was issued after PV_t(j - 1) and its barrier covers both, so O_t is still here.
+      l += row_exp(r, p.scale_log2, m == -INFINITY ? 0.f : m);
+      // PV_t of the step before has read P_t and added to O_t.
+      if (j > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&b.pv_done[t], (steps - 1) & 1, limit, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      tmem_st32(tP, r[0]);
+      tmem_st32(tP + 32, r[1]);
       if (j > 0 && __any_sync(0xffffffffu, need)) {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           uint32_t o[16];
-          tmem_ld16(tO + c * 16, o);
+          tmem_ld16(tO + t * 128 + c * 16, o);
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-          tmem_st16(tO + c * 16, o);
+          tmem_st16(tO + t * 128 + c * 16, o);
         }
       }
       tmem_st_wait();
@@ -372,36 +378,61 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
       mbar_arrive(&b.p_full[t]);
     }
     if (ok && n_kv > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&b.o_done[t], done & 1, limit, abort_flag));
-      ++done;
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.pv_done[t], (steps - 1) & 1, limit, abort_flag));
     }
     if (!ok) break;
     tc_fence_after();
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // a NaN row stays NaN, an empty row gives 0
-    const float lse2 = l > 0.f || l != l ? m + log2f(l) : -INFINITY;
+    float scale_own = 1.f, scale_other = 0.f;
+    if (both) {
+      // Join the two accumulators of the row; each warpgroup then writes half of the columns.
+      exchange[t * 128 + row] = make_float2(m, l);
+      named_bar_sync(2, 256);
+      const float2 other = exchange[(t ^ 1) * 128 + row];
+      const float top = fmaxf(m, other.x);
+      scale_own = m == -INFINITY ? 0.f : ex2(m - top);
+      scale_other = other.x == -INFINITY ? 0.f : ex2(other.x - top);
+      l = t == 0 ? l * scale_own + other.y * scale_other : other.y * scale_other + l * scale_own;
+      m = top;
+    }
+    const bool some = l > 0.f || l != l;            // a NaN row stays NaN, an empty row gives 0
+    const float inv = some ? 1.f / l : 0.f;
+    const float lse2 = some ? m + log2f(l) : -INFINITY;
+    scale_own *= inv;
+    scale_other *= inv;
     const int head = it.head * p.G + g;
-    const long q = static_cast<long>(it.q0) + t * p.bt + tok;
+    const long q = static_cast<long>(it.q0) + first + tok;
     const bool part = it.slot >= 0;
-    const long part_row = (static_cast<long>(it.slot) + t * it.pad) * p.part_rows + row;
+    const long part_row = (static_cast<long>(it.slot) + (w.solo ? 0 : t * it.pad)) * p.part_rows + row;
     const long o_off = part ? part_row * D : (q * p.Hq + head) * D;
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      uint32_t r[16];
-      if (n_kv > 0) {
-        tmem_ld16(tO + c * 16, r);
-        tmem_ld_wait();
-      }
+    constexpr int kPieces = D / 16;
+    const int c0 = both && t == 1 ? kPieces / 2 : 0, c1 = both && t == 0 ? kPieces / 2 : kPieces;
+#pragma unroll 2
+    for (int c = c0; c < c1; ++c) {
       float v[16];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) v[k] = n_kv > 0 && inv != 0.f ? __uint_as_float(r[k]) * inv : 0.f;
-      const long first = o_off + c * 16;
-      if (!live || !H3_IN_BOUNDS(first, first + 15, part ? p.part_extent : p.o_extent, p.status)) continue;
+      for (int k = 0; k < 16; ++k) v[k] = 0.f;
+      if (n_kv > 0) {
+        uint32_t r[16];
+        tmem_ld16(tO + t * 128 + c * 16, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = some ? __uint_as_float(r[k]) * scale_own : 0.f;
+      }
+      if (both) {
+        uint32_t r[16];
+        tmem_ld16(tO + (t ^ 1) * 128 + c * 16, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = some ? fmaf(__uint_as_float(r[k]), scale_other, v[k]) : 0.f;
+      }
+      const long at = o_off + c * 16;
+      if (!live || !H3_IN_BOUNDS(at, at + 15, part ? p.part_extent : p.o_extent, p.status)) continue;
       if (part) {
-        float4* dst = reinterpret_cast<float4*>(p.part_o + first);
+        float4* dst = reinterpret_cast<float4*>(p.part_o + at);
 #pragma unroll
         for (int k = 0; k < 4; ++k) dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
       } else {
-        uint4* dst = reinterpret_cast<uint4*>(p.o + first);
+        uint4* dst = reinterpret_cast<uint4*>(p.o + at);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
           dst[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
@@ -409,12 +440,15 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
       }
     }
     const long lse_off = static_cast<long>(head) * p.Tq + q;
-    if (live && part) {
-      p.part_lse[part_row] = lse2;
-    } else if (live && H3_IN_BOUNDS(lse_off, lse_off, p.lse_extent, p.status)) {
-      p.lse[lse_off] = lse2 * 0.6931471805599453f;
+    if (!both || t == 0) {
+      if (live && part) {
+        p.part_lse[part_row] = lse2;
+      } else if (live && H3_IN_BOUNDS(lse_off, lse_off, p.lse_extent, p.status)) {
+        p.lse[lse_off] = lse2 * 0.6931471805599453f;
+      }
     }
     tc_fence_before();
+    if (both) named_bar_sync(2, 256);    // both accumulators and the exchange are free again
   }
   if (!ok) {
     if (lane_id() == 0) report_status(p.status, kStatusTimeoutAccFull, steps);
@@ -427,22 +461,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ PackedFwdParams p) {
   using C = Fwd<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;
-  uint8_t* ring = sQ + 2 * C::kTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kTile);
+  Ring<C::kK> rk;
+  Ring<C::kV> rv;
+  float2* exchange = reinterpret_cast<float2*>(sQ + (2 + C::kK + C::kV) * C::kTile);   // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 256);
   Bars b;
   b.q_full = bars;
   b.q_empty = bars + 2;
   b.s_full = bars + 4;
   b.p_full = bars + 6;
-  b.o_done = bars + 8;
+  b.pv_done = bars + 8;
   b.drain = bars + 10;
-  b.slot_full = bars + 12;
-  b.slot_empty = b.slot_full + C::kSlots;
-  b.tail_full = b.slot_empty + C::kSlots;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(b.tail_full + C::kSlots);
+  b.s_taken = bars + 12;
+  rk.place(bars + 13, sQ + 2 * C::kTile);
+  rv.place(bars + 13 + rk.kBarriers, rk.base + C::kK * C::kTile);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13 + rk.kBarriers + rv.kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id();
   if (threadIdx.x == 0) {
@@ -451,14 +486,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b.q_empty[t], 1);
       mbar_init(&b.s_full[t], 1);
       mbar_init(&b.p_full[t], 128);
-      mbar_init(&b.o_done[t], 1);
+      mbar_init(&b.pv_done[t], 1);
     }
-    for (int s = 0; s < C::kSlots; ++s) {
-      mbar_init(&b.slot_full[s], 1);
-      mbar_init(&b.slot_empty[s], 1);
-      mbar_init(&b.tail_full[s], 1);
-    }
-    mbar_init(b.drain, 1);
+    rk.init();
+    rv.init();
+    mbar_init(&b.drain[0], 1);
+    mbar_init(&b.drain[1], 1);
+    mbar_init(b.s_taken, 128);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tq);
@@ -476,11 +510,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     setmaxnreg_dec<kRegsLow>();
     if (warp == 0) {
-      if (elect_one()) load_warp<D>(tq, tk, tv, p, sQ, ring, b, abort_flag);
+      if (elect_one()) load_warp<D>(tq, tk, tv, p, sQ, rk, rv, b, abort_flag);
     } else if (warp == 1) {
-      if (elect_one()) mma_warp<D>(p, sQ, ring, b, abort_flag, tmem);
+      if (elect_one()) score_warp<D>(p, sQ, rk, b, abort_flag, tmem);
     } else if (warp == 2) {
-      clean_warp<D>(p, ring, b, abort_flag);
+      clean_warp<D>(p, rv, abort_flag);
+    } else {
+      if (elect_one()) value_warp<D>(p, rv, b, abort_flag, tmem);
     }
     __syncwarp();
     tc_fence_before();
@@ -492,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   setmaxnreg_inc<kRegsHigh>();
-  softmax_warps<D>(p, b, abort_flag, tmem, (warp - 4) >> 2);
+  softmax_warps<D>(p, b, abort_flag, exchange, tmem, (warp - 4) >> 2);
   __syncwarp();
   tc_fence_before();
   named_bar_sync(1, kThreads);

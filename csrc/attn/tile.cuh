@@ -3,6 +3,7 @@
 #pragma once
 
 #include "../common/ptx.cuh"
+#include "packed.h"
 
 namespace h3 {
 
@@ -57,6 +58,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 
+// 32 lanes x 32 bit, 32 consecutive columns per thread (store into TMEM).
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void setmaxnreg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -104,5 +118,93 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int first) {
     for (int i = lane_id(); i < pieces; i += 32)
       *reinterpret_cast<uint4*>(tile + c * kChunkBytes + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
 }
+
+__device__ __forceinline__ PackedItem load_item(const PackedItem* p) {
+  PackedItem it;
+  const int4 a = __ldg(reinterpret_cast<const int4*>(p)), b = __ldg(reinterpret_cast<const int4*>(p) + 1);
+  it.q0 = a.x, it.nq = a.y, it.k0 = a.z, it.nk = a.w, it.diag = b.x, it.head = b.y, it.slot = b.z, it.pad = b.w;
+  return it;
+}
+
+// A ring of tiles.  A tile whose last rows must be zeroed arrives on tail[slot];
+// the cleaning warp then makes the arrival on full[slot].
+template <int SLOTS>
+struct Ring {
+  uint64_t *full, *empty, *tail;
+  uint8_t* base;
+  static constexpr int kBarriers = 3 * SLOTS;
+  __device__ __forceinline__ void place(uint64_t* bars, uint8_t* tiles) {
+    full = bars, empty = bars + SLOTS, tail = bars + 2 * SLOTS, base = tiles;
+  }
+  __device__ __forceinline__ void init() const {
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&tail[s], 1);
+    }
+  }
+  __device__ __forceinline__ static int slot(int n) { return n % SLOTS; }
+  __device__ __forceinline__ bool wait_full(int n, uint64_t limit, volatile int* abort) const {
+    return mbar_wait(&full[n % SLOTS], static_cast<uint32_t>(n / SLOTS) & 1u, limit, abort);
+  }
+};
+
+// The loader's side of a ring.
+template <int SLOTS>
+struct Feed {
+  int n = 0;
+  uint32_t tail_slots = 0, tail_parity = 0;
+  // Waits for the next slot and arms its barrier; null if the wait gave up.
+  __device__ __forceinline__ uint64_t* next(const Ring<SLOTS>& r, bool tail, uint32_t bytes, uint64_t limit,
+                                            volatile int* abort, int& slot) {
+    slot = n % SLOTS;
+    if (!mbar_wait(&r.empty[slot], (static_cast<uint32_t>(n / SLOTS) & 1u) ^ 1u, limit, abort)) return nullptr;
+    uint64_t* full = tail ? &r.tail[slot] : &r.full[slot];
+    tail_slots = (tail_slots & ~(1u << slot)) | (tail ? 1u << slot : 0u);
+    if (tail) tail_parity ^= 1u << slot;
+    mbar_arrive_expect_tx(full, bytes);
+    ++n;
+    return full;
+  }
+  // Never leave a TMA write in flight into this CTA's shared memory.
+  __device__ __forceinline__ void drain(const Ring<SLOTS>& r, uint64_t limit) const {
+    volatile int never = 0;
+    for (int s = 0; s < min(n, SLOTS); ++s) {
+      const int last = (n - 1 - s) / SLOTS * SLOTS + s;
+      if (tail_slots >> s & 1u)
+        mbar_wait(&r.tail[s], (tail_parity >> s & 1u) ^ 1u, limit, &never);
+      else
+        mbar_wait(&r.full[s], static_cast<uint32_t>(last / SLOTS) & 1u, limit, &never);
+    }
+  }
+};
+
+// One tail tile of a ring (all lanes of the cleaning warp).
+template <int CHUNKS, int TILE, int SLOTS>
+__device__ __forceinline__ bool clean_tile(const Ring<SLOTS>& r, int n, int first, uint32_t& parity, uint64_t limit,
+                                           volatile int* abort) {
+  const int slot = n % SLOTS;
+  if (!__all_sync(0xffffffffu, mbar_wait(&r.tail[slot], parity >> slot & 1u, limit, abort))) return false;
+  parity ^= 1u << slot;
+  zero_tile_rows<CHUNKS>(r.base + slot * TILE, first);
+  fence_async_smem();
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(&r.full[slot]);
+  return true;
+}
+
+// The consumer's side of a ring: the slot it reads next.  One thread follows one
+// ring through all its tiles, so it can never be two phases off.
+template <int SLOTS>
+struct Cursor {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == SLOTS) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 }  // namespace h3

@@ -7,18 +7,24 @@
 //   dx   = r * gw - x * r^3 * mean_d(gw * x),   dw = sum over tokens and heads of g * n
 //
 // Every element is read once and written once, so DRAM bandwidth is the bound.
-// A lane group of D / 8 lanes owns one head of one token: a lane holds four
-// rotation pairs in registers (one 16-byte load when pairs are interleaved,
-// two 8-byte loads when they are split by halves), the norm's sums are
-// shuffles inside the group, and x is never read twice.  A block works on a
-// few tokens; it computes their cos / sin once into shared memory and uses
-// them for all query and key heads, so no [T, D/2] tables exist in memory.
-// The weight gradients stay in registers over all tokens of a block
-// (a lane's columns are fixed) and are summed in a fixed order: per block into
-// a partial row, and by a second small kernel over the rows.
+// A warp owns one token (or, in a call of few tokens, a run of its heads): its
+// two lane groups of D / 8 lanes (four groups at D = 64) take heads in turn, a
+// lane holding the same four rotation pairs of every head (one 16-byte load
+// when pairs are interleaved, two 8-byte loads when they are split by halves).
+// So cos, sin and the norm weights of a lane's pairs are computed once and
+// stay in registers over all heads; the norm's sums are shuffles inside a
+// group, x is never read twice, there are no [T, D/2] tables, no shared memory
+// and no barriers.  The loads of the next batch of heads are issued before the
+// current batch is worked on.
+// The weight gradients stay in registers over all tokens of a warp (a lane's
+// columns are fixed) and are summed in a fixed order: per block into a partial
+// row, and by a second small kernel over the rows.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+
+#include <map>
+#include <mutex>
 
 #include "../common/launch.h"
 #include "../common/ptx.cuh"
@@ -29,12 +35,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxAxes = 4;
-constexpr int kUnroll = 4;   // heads whose loads a lane keeps in flight
 
 struct RopeParams {
   long T;
   int Hq, Hk;
-  int tokens;                   // tokens per block and step
+  int runs, run;                // warps per token, heads (of q and k together) per warp
   long q_tok, q_head, k_tok, k_head;        // input strides (elements)
   long dq_tok, dq_head, dk_tok, dk_head;    // gradient input strides (backward)
   const float* positions;       // [T, axes] or null
@@ -151,214 +156,194 @@ __device__ __forceinline__ void turn(const RopeParams& p, long t, int i, float& 
   s = p.sign * (s0 * c1 + c0 * s1);
 }
 
-// Shared memory: cos, sin [tokens][D/2], then the two weights as their pairs' first and second members.
+// cos and sin of a lane's four pairs of token t.  The groups of a warp work on
+// the same token: each computes its share of the four and they exchange.
 template <int D>
-__device__ __forceinline__ void fill_turns(const RopeParams& p, long t0, int ntok, float* cs, float* sn) {
-  for (int i = threadIdx.x; i < ntok * (D / 2); i += kThreads) {
-    float c, s;
-    turn(p, t0 + i / (D / 2), i % (D / 2), c, s);
-    cs[i] = c;
-    sn[i] = s;
+__device__ __forceinline__ void turns(const RopeParams& p, long t, int l, float (&c)[4], float (&s)[4]) {
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kShare = 4 / kGroups;
+  const int g = lane_id() / kLanes;
+  float mc[kShare], ms[kShare];
+#pragma unroll
+  for (int i = 0; i < kShare; ++i) turn(p, t, 4 * l + g * kShare + i, mc[i], ms[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int from = (i / kShare) * kLanes + l;
+    c[i] = __shfl_sync(0xffffffffu, mc[i % kShare], from);
+    s[i] = __shfl_sync(0xffffffffu, ms[i % kShare], from);
   }
 }
 
+// A lane's weights, as the first and second members of its pairs.
 template <int D, bool INTER>
-__device__ __forceinline__ void fill_weights(const void* qw, const void* kw, bool bf16, float* w) {
-  for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
-    const void* src = i < D ? qw : kw;
-    const int d = i % D;
-    float v = 1.f;
-    if (src != nullptr)
-      v = bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(src)[d]) : static_cast<const float*>(src)[d];
-    const int pair = INTER ? d >> 1 : d % (D / 2), second = INTER ? d & 1 : d / (D / 2);
-    w[(i / D) * D + second * (D / 2) + pair] = v;
-  }
-}
-
-__device__ __forceinline__ void read4(const float* p, int l, float (&v)[4]) {
-  const float4 u = *reinterpret_cast<const float4*>(p + 4 * l);
-  v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-}
-
-// The walk over (token, head) items of a block: item g of the block's
-// tokens x (Hq + Hk) heads, then g + groups, ... without a division.
-struct Walk {
-  int tok, head;
-  __device__ __forceinline__ void to(int item, int heads) {
-    tok = item / heads;
-    head = item - tok * heads;
-  }
-  __device__ __forceinline__ void step(int by, int heads) {
-    head += by;
-    while (head >= heads) {
-      head -= heads;
-      ++tok;
+__device__ __forceinline__ void weights(const void* w, bool bf16, int l, float (&a)[4], float (&b)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int first = INTER ? 2 * (4 * l + i) : 4 * l + i, second = INTER ? first + 1 : first + D / 2;
+    if (bf16) {
+      a[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(w)[first]);
+      b[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(w)[second]);
+    } else {
+      a[i] = static_cast<const float*>(w)[first];
+      b[i] = static_cast<const float*>(w)[second];
     }
   }
-};
+}
 
+// Heads [h0, h1) of one token: x -> y (contiguous heads).
 template <typename T, int D, bool INTER, bool NORM>
-__global__ void __launch_bounds__(kThreads)
-    qk_rope_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const void* __restrict__ qw,
-                       const void* __restrict__ kw, T* __restrict__ q_out, T* __restrict__ k_out, RopeParams p) {
-  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes;
-  extern __shared__ __align__(16) float sm[];
-  float* cs = sm;
-  float* sn = cs + p.tokens * (D / 2);
-  float* w = sn + p.tokens * (D / 2);
-  const long t0 = static_cast<long>(blockIdx.x) * p.tokens;
-  const int ntok = static_cast<int>(min(static_cast<long>(p.tokens), p.T - t0));
-  const int heads = p.Hq + p.Hk;
-  // Items are dealt to all blocks of a token group (gridDim.y splits the heads of a short call).
-  const int g = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
-  const int stride = kGroups * gridDim.y;
-  fill_turns<D>(p, t0, ntok, cs, sn);
-  if (NORM) fill_weights<D, INTER>(qw, kw, p.w_bf16, w);
-  __syncthreads();
-  Walk it;
-  it.to(blockIdx.y * kGroups + g, heads);
-  // Lanes of a warp may run out of items at different steps: all of them stay
-  // in the loop (the shuffles are warp-wide) and only skip their accesses.
-  while (__any_sync(0xffffffffu, it.tok < ntok)) {
-    Raw<T> raw[kUnroll];
-    Walk at[kUnroll];
+__device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head, T* __restrict__ y, int h0, int h1,
+                                              const void* w, bool w_bf16, float eps, const float (&c)[4],
+                                              const float (&s)[4]) {
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 4 : 2;
+  const int g = lane_id() / kLanes, l = lane_id() % kLanes;
+  float wa[4], wb[4];
+  if (NORM) weights<D, INTER>(w, w_bf16, l, wa, wb);
+  Raw<T> next[kBatch];
+  auto fetch = [&](int h) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      at[u] = it;
-      if (it.tok < ntok) {
-        const long t = t0 + it.tok;
-        const T* src = it.head < p.Hq ? q + t * p.q_tok + it.head * p.q_head
-                                      : k + t * p.k_tok + (it.head - p.Hq) * p.k_head;
-        raw[u] = load_pairs<D, INTER>(src, l);
-      } else {
-        raw[u] = Raw<T>{};
-      }
-      it.step(stride, heads);
-    }
+    for (int u = 0; u < kBatch; ++u)
+      next[u] = h + u * kGroups + g < h1 ? load_pairs<D, INTER>(x + (h + u * kGroups + g) * head, l) : Raw<T>{};
+  };
+  fetch(h0);
+  for (int h = h0; h < h1; h += kBatch * kGroups) {
+    Raw<T> now[kBatch];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float a[4], b[4];
-      split<INTER>(raw[u], a, b);
-      const bool is_q = at[u].head < p.Hq;
+    for (int u = 0; u < kBatch; ++u) now[u] = next[u];
+    fetch(h + kBatch * kGroups);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      float a[4], b[4], ya[4], yb[4];
+      split<INTER>(now[u], a, b);
       if (NORM) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        const float r = rsqrtf(group_sum<kLanes>(ss) * (1.f / D) + p.eps);
-        float wa[4], wb[4];
-        const float* wh = w + (is_q ? 0 : D);
-        read4(wh, l, wa);
-        read4(wh + D / 2, l, wb);
+        const float r = rsqrtf(group_sum<kLanes>(ss) * (1.f / D) + eps);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           a[i] *= r * wa[i];
           b[i] *= r * wb[i];
         }
       }
-      if (at[u].tok >= ntok) continue;
-      float c[4], s[4], ya[4], yb[4];
-      read4(cs + at[u].tok * (D / 2), l, c);
-      read4(sn + at[u].tok * (D / 2), l, s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         ya[i] = a[i] * c[i] - b[i] * s[i];
         yb[i] = a[i] * s[i] + b[i] * c[i];
       }
-      const long t = t0 + at[u].tok;
-      T* dst = is_q ? q_out + (t * p.Hq + at[u].head) * D : k_out + (t * p.Hk + at[u].head - p.Hq) * D;
-      store_pairs<D, INTER>(dst, l, ya, yb);
+      const int at = h + u * kGroups + g;
+      if (at < h1) store_pairs<D, INTER>(y + at * D, l, ya, yb);
     }
   }
 }
 
-// Backward.  Blocks take token groups in a grid stride, so that each block
-// leaves one partial row [2][D] of the weight gradients.
+template <typename T, int D, bool INTER, bool NORM>
+__global__ void __launch_bounds__(kThreads)
+    qk_rope_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const void* __restrict__ qw,
+                       const void* __restrict__ kw, T* __restrict__ q_out, T* __restrict__ k_out, RopeParams p) {
+  const long warp = static_cast<long>(blockIdx.x) * (kThreads / 32) + warp_id();
+  const long t = warp / p.runs;
+  if (t >= p.T) return;
+  const int h0 = static_cast<int>(warp - t * p.runs) * p.run, h1 = min(h0 + p.run, p.Hq + p.Hk);
+  float c[4], s[4];
+  turns<D>(p, t, lane_id() % (D / 8), c, s);
+  if (h0 < p.Hq)
+    forward_heads<T, D, INTER, NORM>(q + t * p.q_tok, p.q_head, q_out + t * p.Hq * D, h0, min(h1, p.Hq), qw, p.w_bf16,
+                                     p.eps, c, s);
+  if (h1 > p.Hq)
+    forward_heads<T, D, INTER, NORM>(k + t * p.k_tok, p.k_head, k_out + t * p.Hk * D, max(h0 - p.Hq, 0), h1 - p.Hq, kw,
+                                     p.w_bf16, p.eps, c, s);
+}
+
+// Heads [h0, h1) of one token: dy -> dx; adds to the lane's eight columns of the weight gradient.
+template <typename T, int D, bool INTER>
+__device__ __forceinline__ void backward_heads(const T* __restrict__ x, long head, const T* __restrict__ dy,
+                                               long dy_head, T* __restrict__ dx, int h0, int h1, const void* w,
+                                               bool w_bf16, float eps, const float (&c)[4], const float (&s)[4],
+                                               float (&acc)[8]) {
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 2 : 1;
+  const int g = lane_id() / kLanes, l = lane_id() % kLanes;
+  float wa[4], wb[4];
+  weights<D, INTER>(w, w_bf16, l, wa, wb);
+  Raw<T> next_x[kBatch], next_y[kBatch];
+  auto fetch = [&](int h) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int at = h + u * kGroups + g;
+      next_x[u] = at < h1 ? load_pairs<D, INTER>(x + at * head, l) : Raw<T>{};
+      next_y[u] = at < h1 ? load_pairs<D, INTER>(dy + at * dy_head, l) : Raw<T>{};
+    }
+  };
+  fetch(h0);
+  for (int h = h0; h < h1; h += kBatch * kGroups) {
+    Raw<T> now_x[kBatch], now_y[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      now_x[u] = next_x[u];
+      now_y[u] = next_y[u];
+    }
+    fetch(h + kBatch * kGroups);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      float a[4], b[4], ya[4], yb[4], ga[4], gb[4], ss = 0.f, gx = 0.f;
+      split<INTER>(now_x[u], a, b);
+      split<INTER>(now_y[u], ya, yb);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ga[i] = ya[i] * c[i] + yb[i] * s[i];
+        gb[i] = yb[i] * c[i] - ya[i] * s[i];
+        ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+      }
+      // Rows past h1 are zeros: r is finite and everything below is zero.
+      const float r = rsqrtf(group_sum<kLanes>(ss) * (1.f / D) + eps);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[i] *= r;                              // n
+        b[i] *= r;
+        acc[i] = fmaf(ga[i], a[i], acc[i]);
+        acc[4 + i] = fmaf(gb[i], b[i], acc[4 + i]);
+        ga[i] *= wa[i];
+        gb[i] *= wb[i];
+        gx = fmaf(ga[i], a[i], fmaf(gb[i], b[i], gx));
+      }
+      const float mean = group_sum<kLanes>(gx) * (1.f / D);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ya[i] = r * (ga[i] - a[i] * mean);
+        yb[i] = r * (gb[i] - b[i] * mean);
+      }
+      const int at = h + u * kGroups + g;
+      if (at < h1) store_pairs<D, INTER>(dx + at * D, l, ya, yb);
+    }
+  }
+}
+
+// Backward.  Warps take (token, run of heads) in a grid stride, so that each
+// block leaves one partial row [2][D] of the weight gradients.
 template <typename T, int D, bool INTER>
 __global__ void __launch_bounds__(kThreads)
     qk_norm_rope_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const void* __restrict__ qw,
                             const void* __restrict__ kw, const T* __restrict__ dyq, const T* __restrict__ dyk,
                             T* __restrict__ dq, T* __restrict__ dk, float* __restrict__ partial, RopeParams p) {
-  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes, kPer = 2;
-  extern __shared__ __align__(16) float sm[];
-  float* cs = sm;
-  float* sn = cs + p.tokens * (D / 2);
-  float* w = sn + p.tokens * (D / 2);
-  const int heads = p.Hq + p.Hk;
-  const int g = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
+  constexpr int kLanes = D / 8;
+  const int l = lane_id() % kLanes;
   float acc[2][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.f;
-  fill_weights<D, INTER>(qw, kw, p.w_bf16, w);
-  for (long t0 = static_cast<long>(blockIdx.x) * p.tokens; t0 < p.T; t0 += static_cast<long>(gridDim.x) * p.tokens) {
-    const int ntok = static_cast<int>(min(static_cast<long>(p.tokens), p.T - t0));
-    __syncthreads();   // the previous step has read its turns
-    fill_turns<D>(p, t0, ntok, cs, sn);
-    __syncthreads();
-    Walk it;
-    it.to(g, heads);
-    while (__any_sync(0xffffffffu, it.tok < ntok)) {
-      Raw<T> rx[kPer], ry[kPer];
-      Walk at[kPer];
-#pragma unroll
-      for (int u = 0; u < kPer; ++u) {
-        at[u] = it;
-        if (it.tok < ntok) {
-          const long t = t0 + it.tok;
-          const bool is_q = it.head < p.Hq;
-          const int h = is_q ? it.head : it.head - p.Hq;
-          rx[u] = load_pairs<D, INTER>(is_q ? q + t * p.q_tok + h * p.q_head : k + t * p.k_tok + h * p.k_head, l);
-          ry[u] = load_pairs<D, INTER>(is_q ? dyq + t * p.dq_tok + h * p.dq_head : dyk + t * p.dk_tok + h * p.dk_head,
-                                       l);
-        } else {
-          rx[u] = Raw<T>{};
-          ry[u] = Raw<T>{};
-        }
-        it.step(kGroups, heads);
-      }
-#pragma unroll
-      for (int u = 0; u < kPer; ++u) {
-        const bool live = at[u].tok < ntok, is_q = at[u].head < p.Hq;
-        const int tok = live ? at[u].tok : 0;
-        float a[4], b[4], ya[4], yb[4], c[4], s[4], wa[4], wb[4];
-        split<INTER>(rx[u], a, b);
-        split<INTER>(ry[u], ya, yb);
-        read4(cs + tok * (D / 2), l, c);
-        read4(sn + tok * (D / 2), l, s);
-        const float* wh = w + (is_q ? 0 : D);
-        read4(wh, l, wa);
-        read4(wh + D / 2, l, wb);
-        float ga[4], gb[4], ss = 0.f, gx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          ga[i] = ya[i] * c[i] + yb[i] * s[i];
-          gb[i] = yb[i] * c[i] - ya[i] * s[i];
-          ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-          gx = fmaf(ga[i] * wa[i], a[i], fmaf(gb[i] * wb[i], b[i], gx));
-        }
-        ss = group_sum<kLanes>(ss);
-        gx = group_sum<kLanes>(gx);
-        const float r = rsqrtf(ss * (1.f / D) + p.eps);
-        const float coef = r * r * r * (gx * (1.f / D));
-        if (!live) continue;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float na = ga[i] * (a[i] * r), nb = gb[i] * (b[i] * r);
-          acc[0][i] += is_q ? na : 0.f;
-          acc[0][4 + i] += is_q ? nb : 0.f;
-          acc[1][i] += is_q ? 0.f : na;
-          acc[1][4 + i] += is_q ? 0.f : nb;
-          ya[i] = r * (ga[i] * wa[i]) - a[i] * coef;
-          yb[i] = r * (gb[i] * wb[i]) - b[i] * coef;
-        }
-        const long t = t0 + at[u].tok;
-        T* dst = is_q ? dq + (t * p.Hq + at[u].head) * D : dk + (t * p.Hk + at[u].head - p.Hq) * D;
-        store_pairs<D, INTER>(dst, l, ya, yb);
-      }
-    }
+  const long warps = static_cast<long>(gridDim.x) * (kThreads / 32), total = p.T * p.runs;
+  for (long i = static_cast<long>(blockIdx.x) * (kThreads / 32) + warp_id(); i < total; i += warps) {
+    const long t = i / p.runs;
+    const int h0 = static_cast<int>(i - t * p.runs) * p.run, h1 = min(h0 + p.run, p.Hq + p.Hk);
+    float c[4], s[4];
+    turns<D>(p, t, l, c, s);
+    if (h0 < p.Hq)
+      backward_heads<T, D, INTER>(q + t * p.q_tok, p.q_head, dyq + t * p.dq_tok, p.dq_head, dq + t * p.Hq * D, h0,
+                                  min(h1, p.Hq), qw, p.w_bf16, p.eps, c, s, acc[0]);
+    if (h1 > p.Hq)
+      backward_heads<T, D, INTER>(k + t * p.k_tok, p.k_head, dyk + t * p.dk_tok, p.dk_head, dk + t * p.Hk * D,
+                                  max(h0 - p.Hq, 0), h1 - p.Hq, kw, p.w_bf16, p.eps, c, s, acc[1]);
   }
   // Sum the lane groups in a fixed order: groups of a warp by shuffles, then the warps through shared memory.
-  __syncthreads();
-  float* red = sm;   // [warps][2][D]
+  __shared__ float red[kThreads / 32][2 * D];
 #pragma unroll
   for (int side = 0; side < 2; ++side)
 #pragma unroll
@@ -368,13 +353,13 @@ __global__ void __launch_bounds__(kThreads)
       for (int o = kLanes; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       const int pair = 4 * l + (i & 3), second = i >> 2;
       const int d = INTER ? 2 * pair + second : second * (D / 2) + pair;
-      if (lane_id() < kLanes) red[(warp_id() * 2 + side) * D + d] = v;
+      if (lane_id() < kLanes) red[warp_id()][side * D + d] = v;
     }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
     float v = 0.f;
 #pragma unroll
-    for (int wp = 0; wp < kThreads / 32; ++wp) v += red[wp * 2 * D + i];
+    for (int wp = 0; wp < kThreads / 32; ++wp) v += red[wp][i];
     partial[static_cast<long>(blockIdx.x) * 2 * D + i] = v;
   }
 }
@@ -457,6 +442,33 @@ const void* check_weight(const at::Tensor& w, const at::Tensor& q, const char* w
   return w.data_ptr();
 }
 
+// Warps per token.  One warp for a whole token reads each position and turn
+// once; a call of few tokens has too few warps for that and deals the heads
+// over more, down to one batch of loads each.
+void plan_runs(RopeParams& p, int heads, int D) {
+  const int batch = 32 / (D / 8) * 2;
+  const long want = 148L * 64 * 4;      // four rounds of all resident warps
+  const long runs = std::min<long>((heads + batch - 1) / batch, std::max<long>(1, want / p.T));
+  p.run = static_cast<int>((heads + runs - 1) / runs + batch - 1) / batch * batch;
+  p.runs = (heads + p.run - 1) / p.run;
+}
+
+// Blocks of a kernel that the device holds at once (asked once per kernel and device).
+template <typename F>
+int resident_blocks(F* kernel) {
+  static std::mutex lock;
+  static std::map<std::pair<const void*, int>, int> known;
+  const int device = at::cuda::current_device();
+  std::lock_guard<std::mutex> guard(lock);
+  int& blocks = known[{reinterpret_cast<const void*>(kernel), device}];
+  if (blocks == 0) {
+    int per_sm = 1;
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0));
+    blocks = std::max(1, per_sm) * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  }
+  return blocks;
+}
+
 // D, pair order and element type of a call as compile-time values.
 template <typename F>
 void dispatch(const at::Tensor& q, bool interleaved, F&& f) {
@@ -492,28 +504,18 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const at::Tensor& k, co
   auto k_out = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
   const int heads = p.Hq + p.Hk, D = static_cast<int>(q.size(2));
   if (p.T == 0 || heads == 0) return {q_out, k_out};
-  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // Four tokens a block share one pass of cos / sin and one barrier; a call of
-  // few tokens takes one a block and deals the heads over blocks instead.
-  p.tokens = p.T >= 16L * sms ? 4 : 1;
-  const int groups = kThreads / (D / 8);
-  const unsigned split = p.tokens > 1 ? 1u
-                                      : static_cast<unsigned>(std::min<long>((heads + groups - 1) / groups,
-                                                                             std::max<long>(1, 2L * sms / p.T)));
-  const long blocks = (p.T + p.tokens - 1) / p.tokens;
+  plan_runs(p, heads, D);
+  const long blocks = (p.T * p.runs + kThreads / 32 - 1) / (kThreads / 32);
   TORCH_CHECK(blocks < (1L << 31), "too many tokens");
-  const dim3 grid(static_cast<unsigned>(blocks), split);
-  const size_t smem = static_cast<size_t>(p.tokens * D + 2 * D) * sizeof(float);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
   dispatch(q, interleaved, [&](auto* type, auto dim, auto inter) {
     using T = std::remove_pointer_t<decltype(type)>;
     constexpr int kD = decltype(dim)::value;
     constexpr bool kInter = decltype(inter)::value;
     auto args = [&](auto kernel) {
-      kernel<<<grid, kThreads, smem, stream>>>(reinterpret_cast<const T*>(q.data_ptr()),
-                                               reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
-                                               reinterpret_cast<T*>(q_out.data_ptr()),
-                                               reinterpret_cast<T*>(k_out.data_ptr()), p);
+      kernel<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+          reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
+          reinterpret_cast<T*>(q_out.data_ptr()), reinterpret_cast<T*>(k_out.data_ptr()), p);
     };
     if (qw != nullptr) args(qk_rope_fwd_kernel<T, kD, kInter, true>);
     else args(qk_rope_fwd_kernel<T, kD, kInter, false>);
@@ -546,22 +548,17 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q, const at::Tensor& 
     return {dq, dk, zero[0], zero[1]};
   }
   auto dw = at::empty({2, D}, q.options().dtype(at::kFloat));
-  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  p.tokens = p.T >= 16L * sms ? 4 : 1;
-  const size_t smem = sizeof(float) * std::max<size_t>(static_cast<size_t>(p.tokens * D + 2 * D),
-                                                       static_cast<size_t>(kThreads / 32) * 2 * D);
+  plan_runs(p, heads, D);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
   dispatch(q, interleaved, [&](auto* type, auto dim, auto inter) {
     using T = std::remove_pointer_t<decltype(type)>;
     constexpr int kD = decltype(dim)::value;
     constexpr bool kInter = decltype(inter)::value;
     auto kernel = qk_norm_rope_bwd_kernel<T, kD, kInter>;
-    int per_sm = 1;
-    C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, smem));
-    const long steps = (p.T + p.tokens - 1) / p.tokens;
-    const int grid = static_cast<int>(std::min<long>(steps, static_cast<long>(std::max(1, per_sm)) * sms));
+    const long blocks = (p.T * p.runs + kThreads / 32 - 1) / (kThreads / 32);
+    const int grid = static_cast<int>(std::min<long>(blocks, resident_blocks(kernel)));
     auto partial = at::empty({grid, 2 * D}, dw.options());
-    kernel<<<grid, kThreads, smem, stream>>>(
+    kernel<<<grid, kThreads, 0, stream>>>(
         reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
         reinterpret_cast<const T*>(dq_out.data_ptr()), reinterpret_cast<const T*>(dk_out.data_ptr()),
         reinterpret_cast<T*>(dq.data_ptr()), reinterpret_cast<T*>(dk.data_ptr()), partial.data_ptr<float>(), p);
