@@ -17,10 +17,11 @@
 // this step's S is in registers, so the exponentials run beside the products.
 //
 // Both kernels are persistent over a host-balanced list (packed.h), 384 threads:
-// warp 0 TMA loads, warp 1 issues the MMAs, warp 2 zeroes tile rows past a
-// sequence (they belong to the next one and 0 * NaN would leak into the sums),
-// warp 3 (dkv) stages lse2 and delta of the query tile, warps 4..11 softmax:
-// one row a thread, the two warpgroups take 64 columns each.
+// warp 0 TMA loads; warp 1 issues the products (dq: warp 1 S, warp 3 dP and dQ, one
+// thread each); warp 2 zeroes tile rows past a sequence (they belong to the next one
+// and 0 * NaN would leak into the sums) and (dkv) stages lse2 and delta of the
+// query tile; warps 4..11 softmax, one row a thread, the two warpgroups take 64
+// columns each.
 // P and dS are rounded to bf16 (the MMA's operand type); all sums are fp32.
 // TMEM columns: dq   dQ [0,128)  S [128,256)  dP, dS two buffers [256,512)
 //               dkv  dV [0,128)  dK [128,256)  S^T [256,384)  dP^T, then P^T and dS^T [384,512)
@@ -42,7 +43,7 @@ static_assert(128 * kRegsLow + 256 * kRegsHigh == kThreads * kLaunchRegs, "regis
 template <int D>
 struct Bwd {
   static constexpr int kChunks = D / 64;
-  static constexpr int kTile = kChunks * kChunkBytes;
+  static constexpr int kTile = kChunks * kChunkBytes, kTile16 = kTile >> 4;
   // Two resident tiles, a ring of three (read by two products, a step apart) and a ring of two.
   static constexpr int kLong = 3, kShort = 2;
   static constexpr int kTiles = 2 + kLong + kShort;
@@ -51,30 +52,33 @@ struct Bwd {
   static_assert(kSmem <= 232448, "shared memory");
 };
 
+// Descriptors of a tile at `smem` as a K-major operand and as an MN-major right operand; the tiles of a ring
+// follow at kTile16 each.
+__device__ __forceinline__ uint64_t k_major(const uint8_t* smem) { return umma_smem_desc(smem_u32(smem), 16, 1024); }
+__device__ __forceinline__ uint64_t mn_major(const uint8_t* smem) {
+  return umma_smem_desc(smem_u32(smem), kChunkBytes, 1024);
+}
+
 // S-shaped product of two K-major tiles: D[tmem] = A B^T over D columns.
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t d_tmem, const uint8_t* a, const uint8_t* b) {
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint64_t a, uint64_t b) {
   constexpr uint32_t kIdesc = umma_idesc_bf16(128, 128, false, false);
-  const uint32_t sa = smem_u32(a), sb = smem_u32(b);
 #pragma unroll
   for (int ds = 0; ds < D / 16; ++ds) {
-    const uint32_t off = (ds >> 2) * kChunkBytes + (ds & 3) * 32;
-    umma_f16_ss(d_tmem, umma_smem_desc(sa + off, 16, 1024), umma_smem_desc(sb + off, 16, 1024), kIdesc,
-                ds > 0 ? 1u : 0u);
+    const uint64_t off = (ds >> 2) * (kChunkBytes >> 4) + (ds & 3) * 2;
+    umma_f16_ss(d_tmem, a + off, b + off, kIdesc, ds > 0 ? 1u : 0u);
   }
 }
 
 // Accumulating product with the left operand in TMEM (packed bf16; eight
 // columns per 16 of K, the second half of K at column `half`) and an MN-major tile.
 template <int D>
-__device__ __forceinline__ void issue_accum(uint32_t d_tmem, uint32_t a_tmem, uint32_t half, const uint8_t* b,
-                                            bool first) {
+__device__ __forceinline__ void issue_accum(uint32_t d_tmem, uint32_t a_tmem, uint32_t half, uint64_t b, bool first) {
   constexpr uint32_t kIdesc = umma_idesc_bf16(128, D, false, true);
-  const uint32_t sb = smem_u32(b);
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks)
-    umma_f16_ts(d_tmem, a_tmem + (ks >> 2) * half + (ks & 3) * 8, umma_smem_desc(sb + ks * 2048, kChunkBytes, 1024),
-                kIdesc, (!first || ks > 0) ? 1u : 0u);
+    umma_f16_ts(d_tmem, a_tmem + (ks >> 2) * half + (ks & 3) * 8, b + static_cast<uint64_t>(ks * 128), kIdesc,
+                ks > 0 ? 1u : (first ? 0u : 1u));
 }
 
 // COLS TMEM columns of this thread's row -> bf16 row in global memory.
@@ -141,6 +145,9 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(PackedBwdParams p) {
 }
 
 // ---------------------------------------------------------------- dq
+// dp_full, ds_full (and row_full below) are two barriers used in turn: their
+// producer may be up to two steps ahead of a waiting thread, which on one
+// barrier could not be told from none.
 struct DqBars {
   uint64_t *q_full, *do_full, *q_empty, *do_empty, *s_full, *s_read, *dp_full, *ds_full, *dq_full, *drain;
 };
@@ -171,15 +178,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   DqBars b;
   uint64_t* nb = bars + rk.kBarriers + rv.kBarriers;
   b.q_full = nb, b.do_full = nb + 1, b.q_empty = nb + 2, b.do_empty = nb + 3, b.s_full = nb + 4, b.s_read = nb + 5;
-  b.dp_full = nb + 6, b.ds_full = nb + 8, b.dq_full = nb + 9, b.drain = nb + 10;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 11);
+  b.dp_full = nb + 6, b.ds_full = nb + 8, b.dq_full = nb + 10, b.drain = nb + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id();
   const uint64_t limit = p.status.limit_ns;
   if (threadIdx.x == 0) {
     rk.init();
     rv.init();
-    for (int i = 0; i < 11; ++i) mbar_init(nb + i, (nb + i == b.s_read || nb + i == b.ds_full) ? 256 : 1);
+    for (int i = 0; i < 13; ++i)
+      mbar_init(nb + i, nb + i == b.s_read || nb + i == b.ds_full || nb + i == b.ds_full + 1 ? 8 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tq);
@@ -250,54 +258,62 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (q_used > 0) mbar_wait(b.q_full, (q_used - 1) & 1, limit, &never);
       if (do_used > 0) mbar_wait(b.do_full, (do_used - 1) & 1, limit, &never);
     } else if (warp == 1 && elect_one()) {
-      int nk = 0, nv = 0, items = 0, st = 0;
-      bool ok = true, any = false;
+      Cursor<C::kLong> k;
+      uint32_t items = 0, st = 0;
+      bool ok = true;
+      const uint64_t q_desc = k_major(sQ), k_desc = k_major(rk.base);
       for (int i = begin; i < end && ok; ++i) {
-        const PackedItem it = load_item(p.items + i);
         int tail;
-        const int n = key_tiles(it, tail);
-        if (n == 0) continue;
-        auto scores = [&](int j) {
-          if (!rk.wait_full(nk + j, limit, abort_flag)) return false;
-          tc_fence_after();
-          issue_scores<D>(tmem + 128, sQ, rk.base + rk.slot(nk + j) * C::kTile);
-          umma_commit(b.s_full);
-          if (j + 1 == n) umma_commit(b.q_empty);
-          any = true;
-          return true;
-        };
-        auto grads = [&](int j) {
-          if (!rv.wait_full(nv + j, limit, abort_flag)) return false;
-          tc_fence_after();
-          issue_scores<D>(tmem + 256 + ((st + j) & 1) * 128, sDO, rv.base + rv.slot(nv + j) * C::kTile);
-          umma_commit(&b.dp_full[(st + j) & 1]);
-          umma_commit(&rv.empty[rv.slot(nv + j)]);
-          if (j + 1 == n) umma_commit(b.do_empty);
-          return true;
-        };
-        ok = mbar_wait(b.q_full, items & 1, limit, abort_flag) && scores(0) &&
-             mbar_wait(b.do_full, items & 1, limit, abort_flag) && grads(0);
-        for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n) {
-            ok = mbar_wait(b.s_read, (st + j) & 1, limit, abort_flag) && scores(j + 1) && grads(j + 1);
-            if (!ok) break;
-          }
-          ok = mbar_wait(b.ds_full, (st + j) & 1, limit, abort_flag);
+        const int n = key_tiles(load_item(p.items + i), tail);
+        for (int j = 0; j < n; ++j, ++st, k.next()) {
+          ok = mbar_wait(&rk.full[k.slot], k.phase, limit, abort_flag) &&
+               (j > 0 || mbar_wait(b.q_full, items & 1u, limit, abort_flag)) &&
+               (st == 0 || mbar_wait(b.s_read, (st - 1) & 1u, limit, abort_flag));
           if (!ok) break;
           tc_fence_after();
-          issue_accum<D>(tmem, tmem + 256 + ((st + j) & 1) * 128, 64, rk.base + rk.slot(nk + j) * C::kTile, j == 0);
-          umma_commit(&rk.empty[rk.slot(nk + j)]);
+          issue_scores<D>(tmem + 128, q_desc, k_desc + static_cast<uint64_t>(k.slot * C::kTile16));
+          umma_commit(b.s_full);
+          if (j + 1 == n) umma_commit(b.q_empty);
+        }
+        if (n > 0) ++items;
+      }
+      finish_issuer(&b.drain[0], st > 0, ok, static_cast<int>(st), p.status, abort_flag);
+    } else if (warp == 3 && elect_one()) {
+      Cursor<C::kLong> k;
+      Cursor<C::kShort> v;
+      uint32_t items = 0, st = 0, dps = 0;
+      bool ok = true;
+      const uint64_t do_desc = k_major(sDO), v_desc = k_major(rv.base), k_desc = mn_major(rk.base);
+      for (int i = begin; i < end && ok; ++i) {
+        int tail;
+        const int n = key_tiles(load_item(p.items + i), tail);
+        if (n == 0) continue;
+        // dP runs a step ahead in the other buffer: the dS that was there has been used by the product before.
+        auto grads = [&](int j) {
+          if (!mbar_wait(&rv.full[v.slot], v.phase, limit, abort_flag)) return false;
+          tc_fence_after();
+          issue_scores<D>(tmem + 256 + (dps & 1u) * 128, do_desc, v_desc + static_cast<uint64_t>(v.slot * C::kTile16));
+          umma_commit(&b.dp_full[dps & 1u]);
+          umma_commit(&rv.empty[v.slot]);
+          if (j + 1 == n) umma_commit(b.do_empty);
+          ++dps;
+          v.next();
+          return true;
+        };
+        ok = mbar_wait(b.do_full, items & 1u, limit, abort_flag) && grads(0);
+        for (int j = 0; j < n && ok; ++j, ++st, k.next()) {
+          ok = (j + 1 == n || grads(j + 1)) && mbar_wait(&rk.full[k.slot], k.phase, limit, abort_flag) &&
+               mbar_wait(&b.ds_full[st & 1u], (st >> 1) & 1u, limit, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_accum<D>(tmem, tmem + 256 + (st & 1u) * 128, 64, k_desc + static_cast<uint64_t>(k.slot * C::kTile16),
+                         j == 0);
+          umma_commit(&rk.empty[k.slot]);
           if (j + 1 == n) umma_commit(b.dq_full);
         }
-        nk += n, nv += n, st += n;
         ++items;
       }
-      if (!ok) give_up(p.status, abort_flag, kStatusTimeoutFull, nk);
-      if (any) {
-        umma_commit(b.drain);
-        volatile int never = 0;
-        mbar_wait(b.drain, 0, limit, &never);
-      }
+      finish_issuer(&b.drain[1], dps > 0, ok, static_cast<int>(st), p.status, abort_flag);
     } else if (warp == 2) {
       int nk = 0;
       uint32_t parity = 0;
@@ -355,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(tS + 32, s[1]);
       tmem_ld_wait();
       tc_fence_before();
-      mbar_arrive(b.s_read);
+      warp_arrive(b.s_read);
       const int valid = seen - j * 128 - wg * 64;
       const bool cut = __any_sync(0xffffffffu, valid < 64);
       uint64_t pr[2][16];
@@ -393,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_st16(tP + 16, packed[1]);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(b.ds_full);
+      warp_arrive(&b.ds_full[st & 1]);
     }
     if (ok && n > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait(b.dq_full, items & 1, limit, abort_flag));
@@ -413,6 +429,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- dk, dv
+// Zeros in the first `hidden` of a row's 64 values.
+__device__ __forceinline__ void hide(uint64_t (&v)[2][16], int hidden) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      float x, y;
+      unpack2(v[c][k], x, y);
+      v[c][k] = pack2(c * 32 + 2 * k < hidden ? 0.f : x, c * 32 + 2 * k + 1 < hidden ? 0.f : y);
+    }
+}
+
 struct DkvBars {
   uint64_t *k_full, *v_full, *kv_empty, *s_full, *s_read, *dp_full, *ds_full, *acc_full, *row_full, *drain;
 };
@@ -435,8 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   DkvBars b;
   uint64_t* nb = bars + rq.kBarriers + rd.kBarriers;
   b.k_full = nb, b.v_full = nb + 1, b.kv_empty = nb + 2, b.s_full = nb + 3, b.s_read = nb + 4, b.dp_full = nb + 5;
-  b.ds_full = nb + 6, b.acc_full = nb + 7, b.row_full = nb + 8, b.drain = nb + 10;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 11);
+  b.ds_full = nb + 6, b.acc_full = nb + 8, b.row_full = nb + 9, b.drain = nb + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id();
   const uint64_t limit = p.status.limit_ns;
@@ -444,7 +472,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     rq.init();
     rd.init();
-    for (int i = 0; i < 11; ++i) mbar_init(nb + i, (nb + i == b.s_read || nb + i == b.ds_full) ? 256 : 1);
+    for (int i = 0; i < 13; ++i)
+      mbar_init(nb + i, nb + i == b.s_read || nb + i == b.ds_full || nb + i == b.ds_full + 1 ? 8 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tq);
@@ -525,77 +554,66 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(b.v_full, (used - 1) & 1, limit, &never);
       }
     } else if (warp == 1 && elect_one()) {
-      int nt = 0, items = 0;    // query tiles (= steps) so far
-      bool ok = true, any = false;
+      // One thread for all products, in the order dV dK dP' S'' of steps j, j, j + 1,
+      // j + 2: S'' then runs while the softmax warps turn dP' into dS', which
+      // is the one stretch where no other product is ready.
+      Cursor<C::kLong> q, q_ahead;      // tiles of the next dK and of the next S
+      Cursor<C::kShort> d, d_ahead;     // tiles of the next dV and of the next dP
+      uint32_t st = 0, scored = 0;      // steps used up, steps scored
+      bool ok = true;
+      const uint64_t k_desc = k_major(sK), qk_desc = k_major(rq.base), qm_desc = mn_major(rq.base);
+      const uint64_t v_desc = k_major(sV), dk_desc = k_major(rd.base), dm_desc = mn_major(rd.base);
+      uint32_t items = 0;
       for (int i = begin; i < end && ok; ++i) {
-        const PackedItem it = load_item(p.items + i);
         int last_rows;
-        const int n = query_tiles(it, last_rows);
+        const int n = query_tiles(load_item(p.items + i), last_rows);
         if (n == 0) continue;
-        auto scores = [&](int j) {
-          if (!rq.wait_full(nt + j, limit, abort_flag)) return false;
+        auto scores = [&]() {
+          if (!mbar_wait(&rq.full[q_ahead.slot], q_ahead.phase, limit, abort_flag) ||
+              (scored > 0 && !mbar_wait(b.s_read, (scored - 1) & 1u, limit, abort_flag)))
+            return false;
           tc_fence_after();
-          issue_scores<D>(tmem + 256, sK, rq.base + rq.slot(nt + j) * C::kTile);
+          issue_scores<D>(tmem + 256, k_desc, qk_desc + static_cast<uint64_t>(q_ahead.slot * C::kTile16));
           umma_commit(b.s_full);
-          any = true;
+          q_ahead.next();
+          ++scored;
           return true;
         };
-        auto grads = [&](int j) {
-          if (!rd.wait_full(nt + j, limit, abort_flag)) return false;
+        auto grads = [&]() {
+          if (!mbar_wait(&rd.full[d_ahead.slot], d_ahead.phase, limit, abort_flag)) return false;
           tc_fence_after();
-          issue_scores<D>(tmem + 384, sV, rd.base + rd.slot(nt + j) * C::kTile);
+          issue_scores<D>(tmem + 384, v_desc, dk_desc + static_cast<uint64_t>(d_ahead.slot * C::kTile16));
           umma_commit(b.dp_full);
+          d_ahead.next();
           return true;
         };
-        ok = mbar_wait(b.k_full, items & 1, limit, abort_flag) && scores(0) &&
-             mbar_wait(b.v_full, items & 1, limit, abort_flag) && grads(0);
-        for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n) {
-            ok = mbar_wait(b.s_read, (nt + j) & 1, limit, abort_flag) && scores(j + 1);
-            if (!ok) break;
-          }
-          ok = mbar_wait(b.ds_full, (nt + j) & 1, limit, abort_flag);
+        ok = mbar_wait(b.k_full, items & 1u, limit, abort_flag) && scores() &&
+             mbar_wait(b.v_full, items & 1u, limit, abort_flag) && grads() && (n == 1 || scores());
+        for (int j = 0; j < n && ok; ++j, ++st, q.next(), d.next()) {
+          ok = mbar_wait(&b.ds_full[st & 1u], (st >> 1) & 1u, limit, abort_flag);
           if (!ok) break;
           tc_fence_after();
           // P^T of the two warpgroups at columns 384 and 448, dS^T at 416 and 480.
-          issue_accum<D>(tmem, tmem + 384, 64, rd.base + rd.slot(nt + j) * C::kTile, j == 0);
-          umma_commit(&rd.empty[rd.slot(nt + j)]);
-          issue_accum<D>(tmem + 128, tmem + 416, 64, rq.base + rq.slot(nt + j) * C::kTile, j == 0);
-          umma_commit(&rq.empty[rq.slot(nt + j)]);
+          issue_accum<D>(tmem, tmem + 384, 64, dm_desc + static_cast<uint64_t>(d.slot * C::kTile16), j == 0);
+          umma_commit(&rd.empty[d.slot]);
+          issue_accum<D>(tmem + 128, tmem + 416, 64, qm_desc + static_cast<uint64_t>(q.slot * C::kTile16), j == 0);
+          umma_commit(&rq.empty[q.slot]);
+          // The next dP overwrites P^T and dS^T: one thread's products run in order.
           if (j + 1 < n) {
-            ok = grads(j + 1);
+            ok = grads() && (j + 2 == n || scores());
           } else {
             umma_commit(b.acc_full);
             umma_commit(b.kv_empty);
           }
         }
-        nt += n;
         ++items;
       }
-      if (!ok) give_up(p.status, abort_flag, kStatusTimeoutFull, nt);
-      if (any) {
-        umma_commit(b.drain);
-        volatile int never = 0;
-        mbar_wait(b.drain, 0, limit, &never);
-      }
+      finish_issuer(&b.drain[0], scored > 0, ok, static_cast<int>(st), p.status, abort_flag);
     } else if (warp == 2) {
-      int nt = 0;
-      uint32_t pq = 0, pd = 0;
-      for (int i = begin; i < end; ++i) {
-        const PackedItem it = load_item(p.items + i);
-        int last_rows;
-        const int n = query_tiles(it, last_rows);
-        if (n > 0 && last_rows < rows_full &&
-            (!clean_tile<C::kChunks, C::kTile>(rq, nt + n - 1, last_rows, pq, limit, abort_flag) ||
-             !clean_tile<C::kChunks, C::kTile>(rd, nt + n - 1, last_rows, pd, limit, abort_flag))) {
-          if (lane_id() == 0) give_up(p.status, abort_flag, kStatusTimeoutFull, i);
-          break;
-        }
-        nt += n;
-      }
-    } else if (warp == 3) {
-      // lse2 and delta of each query tile; rows past the tile's tokens weigh nothing.
+      // -lse2 and -delta of each query tile (rows past the tile's tokens weigh
+      // nothing), and zeros in the last tile's rows that no query of the item has.
       int st = 0;
+      uint32_t pq = 0, pd = 0;
       bool ok = true;
       for (int i = begin; i < end && ok; ++i) {
         const PackedItem it = load_item(p.items + i);
@@ -608,11 +626,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int r = k * 32 + lane_id();
-            a[k] = r < rows ? p.lse2[at + r] : INFINITY;
-            d[k] = r < rows ? p.delta[at + r] : 0.f;
+            a[k] = r < rows ? -p.lse2[at + r] : -INFINITY;
+            d[k] = r < rows ? -p.delta[at + r] : 0.f;
           }
           // The stage is free once the step before last has been used up.
-          ok = __all_sync(0xffffffffu, st < 2 || mbar_wait(b.ds_full, st & 1, limit, abort_flag));
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.ds_full[st & 1], ((st >> 1) & 1) ^ 1, limit, abort_flag));
           if (!ok) break;
           float* dst = sRow + (st & 1) * 256;
 #pragma unroll
@@ -623,6 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane_id() == 0) mbar_arrive(&b.row_full[st & 1]);
         }
+        if (ok && n > 0 && last_rows < rows_full)
+          ok = clean_tile<C::kChunks, C::kTile>(rq, st - 1, last_rows, pq, limit, abort_flag) &&
+               clean_tile<C::kChunks, C::kTile>(rd, st - 1, last_rows, pd, limit, abort_flag);
       }
       if (!ok && lane_id() == 0) give_up(p.status, abort_flag, kStatusTimeoutEmpty, st);
     }
@@ -659,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(tS + 32, s[1]);
       tmem_ld_wait();
       tc_fence_before();
-      mbar_arrive(b.s_read);
+      warp_arrive(b.s_read);
       // Columns are token * G + head: the tokens before key - diag do not see this key.
       const int hidden = max(0, row - it.diag - j * p.bt) * p.G - wg * 64;
       const bool cut = __any_sync(0xffffffffu, hidden > 0);
@@ -668,23 +689,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float4 l = *reinterpret_cast<const float4*>(rs + c * 32 + 4 * k);
+          const ulonglong2 neg_lse = *reinterpret_cast<const ulonglong2*>(rs + c * 32 + 4 * k);   // two pairs
           float x, y, z, w;
-          unpack2(fma2(pack2(__uint_as_float(s[c][4 * k]), __uint_as_float(s[c][4 * k + 1])), scale2, pack2(-l.x, -l.y)),
-                  x, y);
-          unpack2(fma2(pack2(__uint_as_float(s[c][4 * k + 2]), __uint_as_float(s[c][4 * k + 3])), scale2,
-                       pack2(-l.z, -l.w)),
-                  z, w);
-          x = ex2(x), y = ex2(y), z = ex2(z), w = ex2(w);
-          if (cut) {
-            const int at = c * 32 + 4 * k;
-            x = at < hidden ? 0.f : x;
-            y = at + 1 < hidden ? 0.f : y;
-            z = at + 2 < hidden ? 0.f : z;
-            w = at + 3 < hidden ? 0.f : w;
-          }
-          pr[c][2 * k] = pack2(x, y);
-          pr[c][2 * k + 1] = pack2(z, w);
+          unpack2(fma2(pack2(__uint_as_float(s[c][4 * k]), __uint_as_float(s[c][4 * k + 1])), scale2, neg_lse.x), x, y);
+          unpack2(fma2(pack2(__uint_as_float(s[c][4 * k + 2]), __uint_as_float(s[c][4 * k + 3])), scale2, neg_lse.y), z,
+                  w);
+          pr[c][2 * k] = pack2(ex2(x), ex2(y));
+          pr[c][2 * k + 1] = pack2(ex2(z), ex2(w));
+        }
+      if (cut) hide(pr, hidden);
+      uint32_t pp[2][16];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float x, y;
+          unpack2(pr[c][k], x, y);
+          pp[c][k] = pack_bf16x2(x, y);
         }
       ok = __all_sync(0xffffffffu, mbar_wait(b.dp_full, st & 1, limit, abort_flag));
       if (!ok) break;
@@ -696,37 +717,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       // This warpgroup's dP columns are read: P^T goes over the first half of them, dS^T over the second.
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t pp[16], pd[16];
+        tmem_st16(tP + c * 16, pp[c]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float4 d = *reinterpret_cast<const float4*>(rs + 128 + c * 32 + 4 * k);
-          float x, y, z, w;
-          unpack2(pr[c][2 * k], x, y);
-          unpack2(pr[c][2 * k + 1], z, w);
-          pp[2 * k] = pack_bf16x2(x, y);
-          pp[2 * k + 1] = pack_bf16x2(z, w);
-          unpack2(mul2(pr[c][2 * k], add2(pack2(__uint_as_float(dp[c][4 * k]), __uint_as_float(dp[c][4 * k + 1])),
-                                          pack2(-d.x, -d.y))),
-                  x, y);
-          unpack2(mul2(pr[c][2 * k + 1], add2(pack2(__uint_as_float(dp[c][4 * k + 2]), __uint_as_float(dp[c][4 * k + 3])),
-                                              pack2(-d.z, -d.w))),
-                  z, w);
-          if (cut) {   // a select, not a product: what a masked place holds may be NaN
-            const int at = c * 32 + 4 * k;
-            x = at < hidden ? 0.f : x;
-            y = at + 1 < hidden ? 0.f : y;
-            z = at + 2 < hidden ? 0.f : z;
-            w = at + 3 < hidden ? 0.f : w;
-          }
-          pd[2 * k] = pack_bf16x2(x, y);
-          pd[2 * k + 1] = pack_bf16x2(z, w);
+          const ulonglong2 neg_delta = *reinterpret_cast<const ulonglong2*>(rs + 128 + c * 32 + 4 * k);
+          pr[c][2 * k] = mul2(pr[c][2 * k], add2(pack2(__uint_as_float(dp[c][4 * k]), __uint_as_float(dp[c][4 * k + 1])),
+                                                 neg_delta.x));
+          pr[c][2 * k + 1] = mul2(pr[c][2 * k + 1], add2(pack2(__uint_as_float(dp[c][4 * k + 2]),
+                                                               __uint_as_float(dp[c][4 * k + 3])),
+                                                         neg_delta.y));
         }
-        tmem_st16(tP + c * 16, pp);
+      }
+      if (cut) hide(pr, hidden);   // zeros, not products: what a masked place holds may be NaN
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pd[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float x, y;
+          unpack2(pr[c][k], x, y);
+          pd[k] = pack_bf16x2(x, y);
+        }
         tmem_st16(tP + 32 + c * 16, pd);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(b.ds_full);
+      warp_arrive(&b.ds_full[st & 1]);
     }
     if (ok && n > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait(b.acc_full, items & 1, limit, abort_flag));

@@ -150,20 +150,6 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorM
     if (q_used[t] > 0) mbar_wait(&b.q_full[t], (q_used[t] - 1) & 1, limit, &never);
 }
 
-// Ends an issuer: no product of this thread may still read shared memory or TMEM.
-__device__ __forceinline__ void finish_issuer(uint64_t* drain, bool any, bool ok, int where, const KernelStatus& st,
-                                              volatile int* abort_flag) {
-  if (!ok) {
-    report_status(st, kStatusTimeoutFull, where);
-    *abort_flag = 1;
-  }
-  if (any) {
-    umma_commit(drain);
-    volatile int never = 0;
-    mbar_wait(drain, 0, st.limit_ns, &never);
-  }
-}
-
 // All scores, in the order (key tile, warpgroup).
 template <int D>
 __device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kK>& rk, const Bars& b,
@@ -336,7 +322,7 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
       for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
       tmem_ld_wait();
       tc_fence_before();
-      mbar_arrive(b.s_taken);
+      warp_arrive(b.s_taken);
       const int valid = seen - w.key_tile(t, j) * 128;
       if (__any_sync(0xffffffffu, valid < 128)) {
 #pragma unroll
@@ -375,7 +361,7 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&b.p_full[t]);
+      warp_arrive(&b.p_full[t]);
     }
     if (ok && n_kv > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait(&b.pv_done[t], (steps - 1) & 1, limit, abort_flag));
@@ -485,14 +471,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b.q_full[t], 1);
       mbar_init(&b.q_empty[t], 1);
       mbar_init(&b.s_full[t], 1);
-      mbar_init(&b.p_full[t], 128);
+      mbar_init(&b.p_full[t], 4);
       mbar_init(&b.pv_done[t], 1);
     }
     rk.init();
     rv.init();
     mbar_init(&b.drain[0], 1);
     mbar_init(&b.drain[1], 1);
-    mbar_init(b.s_taken, 128);
+    mbar_init(b.s_taken, 4);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tq);

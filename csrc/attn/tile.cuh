@@ -84,6 +84,12 @@ __device__ __forceinline__ void named_bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// One arrival for the whole warp (32 on one address would be taken one by one).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(bar);
+}
+
 // Generic-proxy writes to shared memory become visible to the async proxy (MMA operands, TMA).
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -142,10 +148,6 @@ struct Ring {
       mbar_init(&empty[s], 1);
       mbar_init(&tail[s], 1);
     }
-  }
-  __device__ __forceinline__ static int slot(int n) { return n % SLOTS; }
-  __device__ __forceinline__ bool wait_full(int n, uint64_t limit, volatile int* abort) const {
-    return mbar_wait(&full[n % SLOTS], static_cast<uint32_t>(n / SLOTS) & 1u, limit, abort);
   }
 };
 
@@ -206,5 +208,19 @@ struct Cursor {
     }
   }
 };
+
+// Ends an issuer: no product of this thread may still read shared memory or TMEM.
+__device__ __forceinline__ void finish_issuer(uint64_t* drain, bool any, bool ok, int where, const KernelStatus& st,
+                                              volatile int* abort_flag) {
+  if (!ok) {
+    report_status(st, kStatusTimeoutFull, where);
+    *abort_flag = 1;
+  }
+  if (any) {
+    umma_commit(drain);
+    volatile int never = 0;
+    mbar_wait(drain, 0, st.limit_ns, &never);
+  }
+}
 
 }  // namespace h3
