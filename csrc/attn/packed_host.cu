@@ -1,6 +1,7 @@
 // Host side of attention over packed sequences: the work lists and the launches.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -235,6 +236,20 @@ CUtensorMap query_map(const at::Tensor& t, int group, int bt) {
   return encode(t, 4, dims, strides, box);
 }
 
+// `t` itself if TMA and the kernels can read its layout (unit stride within a
+// head, every head on a 16-byte boundary, no zero stride), else a contiguous copy.
+at::Tensor fit(const at::Tensor& t) {
+  if (!t.is_cuda() || t.dim() != 3 || t.numel() == 0 || t.scalar_type() != at::kBFloat16) return t;
+  const bool fits = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                    (t.size(0) == 1 || (t.stride(0) > 0 && t.stride(0) % 8 == 0)) &&
+                    (t.size(1) == 1 || (t.stride(1) > 0 && t.stride(1) % 8 == 0));
+  return fits ? t : t.contiguous();
+}
+
+at::Tensor empty_cuda(at::IntArrayRef sizes, c10::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+
 void check_rows(const at::Tensor& t, const char* what, int64_t tokens, int64_t heads, int64_t head_dim,
                 const at::Device& device) {
   TORCH_CHECK(t.is_cuda() && t.device() == device, what, " must be a CUDA tensor on q's device");
@@ -377,9 +392,10 @@ std::tuple<at::Tensor, std::vector<int64_t>> packed_schedule(const std::vector<i
   return {t, meta};
 }
 
-std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                              const at::Tensor& blob, const std::vector<int64_t>& meta, double scale,
                                              const at::Tensor& status, int64_t limit_ns) {
+  const at::Tensor q = fit(q_in), k = fit(k_in), v = fit(v_in);
   check_plan(q, blob, meta);
   check_rows(q, "q", meta[kTq], meta[kHq], meta[kD], q.device());
   check_rows(k, "k", meta[kTk], meta[kHk], meta[kD], q.device());
@@ -387,8 +403,8 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q, const at::Tens
   check_scale(scale);
   check_status_word(status, q);
   c10::cuda::CUDAGuard guard(q.get_device());
-  auto o = at::empty({meta[kTq], meta[kHq], meta[kD]}, q.options());
-  auto lse = at::empty({meta[kHq], meta[kTq]}, q.options().dtype(at::kFloat));
+  auto o = empty_cuda({meta[kTq], meta[kHq], meta[kD]}, at::kBFloat16, q);
+  auto lse = empty_cuda({meta[kHq], meta[kTq]}, at::kFloat, q);
   if (meta[kTq] == 0) return {o, lse};
   if (meta[kTk] == 0) {   // nothing to attend to
     o.zero_();
@@ -415,7 +431,7 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q, const at::Tens
   p.status.limit_ns = static_cast<uint64_t>(limit_ns);
   if (meta[kJoinCount] > 0) {
     const int64_t rows = meta[kSlots] * meta[kPartRows];
-    parts = at::empty({rows * (head_dim + 1)}, lse.options());
+    parts = empty_cuda({rows * (head_dim + 1)}, at::kFloat, q);
     p.part_o = parts.data_ptr<float>();
     p.part_lse = p.part_o + rows * head_dim;
     p.part_rows = static_cast<int>(meta[kPartRows]);
@@ -433,11 +449,12 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q, const at::Tens
   return {o, lse};
 }
 
-std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                             const at::Tensor& o, const at::Tensor& lse, const at::Tensor& dout,
+std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                             const at::Tensor& o_in, const at::Tensor& lse, const at::Tensor& do_in,
                                              const at::Tensor& blob, const std::vector<int64_t>& meta, double scale,
                                              const at::Tensor& status, int64_t limit_ns,
                                              const std::vector<at::Tensor>& out) {
+  const at::Tensor q = fit(q_in), k = fit(k_in), v = fit(v_in), o = fit(o_in), dout = fit(do_in);
   check_plan(q, blob, meta);
   const int64_t tq = meta[kTq], tk = meta[kTk], hq = meta[kHq], hk = meta[kHk], d = meta[kD];
   check_rows(q, "q", tq, hq, d, q.device());
@@ -454,7 +471,8 @@ std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q, const at::Tens
   c10::cuda::CUDAGuard guard(q.get_device());
   std::vector<at::Tensor> grads = out;
   if (grads.empty())
-    grads = {at::empty({tq, hq, d}, q.options()), at::empty({tk, hk, d}, q.options()), at::empty({tk, hk, d}, q.options())};
+    grads = {empty_cuda({tq, hq, d}, at::kBFloat16, q), empty_cuda({tk, hk, d}, at::kBFloat16, q),
+             empty_cuda({tk, hk, d}, at::kBFloat16, q)};
   check_rows(grads[0], "dq", tq, hq, d, q.device());
   check_rows(grads[1], "dk", tk, hk, d, q.device());
   check_rows(grads[2], "dv", tk, hk, d, q.device());
@@ -465,7 +483,7 @@ std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q, const at::Tens
   configure_once<packed_bwd_configure>();
   const int32_t* ints = blob.data_ptr<int32_t>();
   const int head_dim = static_cast<int>(d);
-  auto rows = at::empty({2, hq * tq}, lse.options());
+  auto rows = empty_cuda({2, hq * tq}, at::kFloat, q);
   PackedBwdParams p{};
   p.G = static_cast<int>(hq / hk);
   p.bt = 128 / p.G;

@@ -21,6 +21,7 @@
 // row, and by a second small kernel over the rows.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <map>
@@ -192,12 +193,11 @@ __device__ __forceinline__ void weights(const void* w, bool bf16, int l, float (
 // Heads [h0, h1) of one token: x -> y (contiguous heads).
 template <typename T, int D, bool INTER, bool NORM>
 __device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head, T* __restrict__ y, int h0, int h1,
-                                              const void* w, bool w_bf16, float eps, const float (&c)[4],
-                                              const float (&s)[4]) {
+                                              const void* w, const RopeParams& p, long t, bool& turned, float (&c)[4],
+                                              float (&s)[4]) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 4 : 2;
   const int g = lane_id() / kLanes, l = lane_id() % kLanes;
   float wa[4], wb[4];
-  if (NORM) weights<D, INTER>(w, w_bf16, l, wa, wb);
   Raw<T> next[kBatch];
   auto fetch = [&](int h) {
 #pragma unroll
@@ -205,6 +205,9 @@ __device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head
       next[u] = h + u * kGroups + g < h1 ? load_pairs<D, INTER>(x + (h + u * kGroups + g) * head, l) : Raw<T>{};
   };
   fetch(h0);
+  if (NORM) weights<D, INTER>(w, p.w_bf16, l, wa, wb);
+  if (!turned) turns<D>(p, t, l, c, s);      // after the first loads are on their way
+  turned = true;
   for (int h = h0; h < h1; h += kBatch * kGroups) {
     Raw<T> now[kBatch];
 #pragma unroll
@@ -218,7 +221,7 @@ __device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        const float r = rsqrtf(group_sum<kLanes>(ss) * (1.f / D) + eps);
+        const float r = rsqrtf(group_sum<kLanes>(ss) * (1.f / D) + p.eps);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           a[i] *= r * wa[i];
@@ -245,25 +248,24 @@ __global__ void __launch_bounds__(kThreads)
   if (t >= p.T) return;
   const int h0 = static_cast<int>(warp - t * p.runs) * p.run, h1 = min(h0 + p.run, p.Hq + p.Hk);
   float c[4], s[4];
-  turns<D>(p, t, lane_id() % (D / 8), c, s);
+  bool turned = false;
   if (h0 < p.Hq)
-    forward_heads<T, D, INTER, NORM>(q + t * p.q_tok, p.q_head, q_out + t * p.Hq * D, h0, min(h1, p.Hq), qw, p.w_bf16,
-                                     p.eps, c, s);
+    forward_heads<T, D, INTER, NORM>(q + t * p.q_tok, p.q_head, q_out + t * p.Hq * D, h0, min(h1, p.Hq), qw, p, t,
+                                     turned, c, s);
   if (h1 > p.Hq)
     forward_heads<T, D, INTER, NORM>(k + t * p.k_tok, p.k_head, k_out + t * p.Hk * D, max(h0 - p.Hq, 0), h1 - p.Hq, kw,
-                                     p.w_bf16, p.eps, c, s);
+                                     p, t, turned, c, s);
 }
 
 // Heads [h0, h1) of one token: dy -> dx; adds to the lane's eight columns of the weight gradient.
 template <typename T, int D, bool INTER>
 __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long head, const T* __restrict__ dy,
                                                long dy_head, T* __restrict__ dx, int h0, int h1, const void* w,
-                                               bool w_bf16, float eps, const float (&c)[4], const float (&s)[4],
-                                               float (&acc)[8]) {
+                                               const RopeParams& p, long t, bool& turned, float (&c)[4],
+                                               float (&s)[4], float (&acc)[8]) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 2 : 1;
   const int g = lane_id() / kLanes, l = lane_id() % kLanes;
   float wa[4], wb[4];
-  weights<D, INTER>(w, w_bf16, l, wa, wb);
   Raw<T> next_x[kBatch], next_y[kBatch];
   auto fetch = [&](int h) {
 #pragma unroll
@@ -274,6 +276,9 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
     }
   };
   fetch(h0);
+  weights<D, INTER>(w, p.w_bf16, l, wa, wb);
+  if (!turned) turns<D>(p, t, l, c, s);
+  turned = true;
   for (int h = h0; h < h1; h += kBatch * kGroups) {
     Raw<T> now_x[kBatch], now_y[kBatch];
 #pragma unroll
@@ -292,24 +297,22 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
         ga[i] = ya[i] * c[i] + yb[i] * s[i];
         gb[i] = yb[i] * c[i] - ya[i] * s[i];
         ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+        gx = fmaf(ga[i] * wa[i], a[i], fmaf(gb[i] * wb[i], b[i], gx));
       }
+      // Both sums before r is known, so that their shuffles overlap.
+      ss = group_sum<kLanes>(ss);
+      gx = group_sum<kLanes>(gx);
       // Rows past h1 are zeros: r is finite and everything below is zero.
-      const float r = rsqrtf(group_sum<kLanes>(ss) * (1.f / D) + eps);
+      const float r = rsqrtf(ss * (1.f / D) + p.eps);
+      const float coef = r * r * (gx * (1.f / D));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        a[i] *= r;                              // n
-        b[i] *= r;
+        ga[i] *= r;
+        gb[i] *= r;
         acc[i] = fmaf(ga[i], a[i], acc[i]);
         acc[4 + i] = fmaf(gb[i], b[i], acc[4 + i]);
-        ga[i] *= wa[i];
-        gb[i] *= wb[i];
-        gx = fmaf(ga[i], a[i], fmaf(gb[i], b[i], gx));
-      }
-      const float mean = group_sum<kLanes>(gx) * (1.f / D);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ya[i] = r * (ga[i] - a[i] * mean);
-        yb[i] = r * (gb[i] - b[i] * mean);
+        ya[i] = ga[i] * wa[i] - a[i] * (r * coef);
+        yb[i] = gb[i] * wb[i] - b[i] * (r * coef);
       }
       const int at = h + u * kGroups + g;
       if (at < h1) store_pairs<D, INTER>(dx + at * D, l, ya, yb);
@@ -334,13 +337,13 @@ __global__ void __launch_bounds__(kThreads)
     const long t = i / p.runs;
     const int h0 = static_cast<int>(i - t * p.runs) * p.run, h1 = min(h0 + p.run, p.Hq + p.Hk);
     float c[4], s[4];
-    turns<D>(p, t, l, c, s);
+    bool turned = false;
     if (h0 < p.Hq)
       backward_heads<T, D, INTER>(q + t * p.q_tok, p.q_head, dyq + t * p.dq_tok, p.dq_head, dq + t * p.Hq * D, h0,
-                                  min(h1, p.Hq), qw, p.w_bf16, p.eps, c, s, acc[0]);
+                                  min(h1, p.Hq), qw, p, t, turned, c, s, acc[0]);
     if (h1 > p.Hq)
       backward_heads<T, D, INTER>(k + t * p.k_tok, p.k_head, dyk + t * p.dk_tok, p.dk_head, dk + t * p.Hk * D,
-                                  max(h0 - p.Hq, 0), h1 - p.Hq, kw, p.w_bf16, p.eps, c, s, acc[1]);
+                                  max(h0 - p.Hq, 0), h1 - p.Hq, kw, p, t, turned, c, s, acc[1]);
   }
   // Sum the lane groups in a fixed order: groups of a warp by shuffles, then the warps through shared memory.
   __shared__ float red[kThreads / 32][2 * D];
@@ -365,18 +368,20 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // dw[i] = sum over rows of partial[row][i]: 32 columns x 32 row slices per block, fixed order.
-__global__ void __launch_bounds__(1024) sum_partials_kernel(const float* __restrict__ partial, int rows, int cols,
-                                                            float* __restrict__ out) {
+__global__ void __launch_bounds__(1024) sum_partials_kernel(const float* __restrict__ partial, int rows, int D,
+                                                            float* __restrict__ dqw, float* __restrict__ dkw) {
   __shared__ float s[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
-  for (int r = threadIdx.y; r < rows; r += 32) v += partial[static_cast<long>(r) * cols + c];
+#pragma unroll 8
+  for (int r = threadIdx.y; r < rows; r += 32) v += partial[static_cast<long>(r) * 2 * D + c];
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   v = s[threadIdx.x][threadIdx.y];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (threadIdx.x == 0) out[blockIdx.x * 32 + threadIdx.y] = v;
+  const int col = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0) (col < D ? dqw[col] : dkw[col - D]) = v;
 }
 
 void check_heads(const at::Tensor& t, const char* what, const at::Tensor& q) {
@@ -389,6 +394,21 @@ void check_heads(const at::Tensor& t, const char* what, const at::Tensor& q) {
                                  (t.size(1) == 1 || t.stride(1) % unit == 0) &&
                                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
               what, " must have unit stride within a head and heads on 16-byte boundaries");
+}
+
+// `t` itself if the kernels can read its layout (unit stride within a head,
+// every head on a 16-byte boundary, no zero stride), else a contiguous copy.
+at::Tensor fit(const at::Tensor& t) {
+  if (!t.is_cuda() || t.dim() != 3 || t.numel() == 0) return t;
+  const int64_t unit = 16 / t.element_size();
+  const bool fits = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                    (t.size(0) == 1 || (t.stride(0) > 0 && t.stride(0) % unit == 0)) &&
+                    (t.size(1) == 1 || (t.stride(1) > 0 && t.stride(1) % unit == 0));
+  return fits ? t : t.contiguous();
+}
+
+at::Tensor empty_cuda(at::IntArrayRef sizes, c10::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
 RopeParams make_params(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& positions,
@@ -443,11 +463,13 @@ const void* check_weight(const at::Tensor& w, const at::Tensor& q, const char* w
 }
 
 // Warps per token.  One warp for a whole token reads each position and turn
-// once; a call of few tokens has too few warps for that and deals the heads
-// over more, down to one batch of loads each.
-void plan_runs(RopeParams& p, int heads, int D) {
-  const int batch = 32 / (D / 8) * 2;
-  const long want = 148L * 64 * 4;      // four rounds of all resident warps
+// once and keeps its loads running from batch to batch (16,411 tokens of 40 heads
+// forward: 70 us with two runs of 20 heads, whose last batches are half empty); a
+// call with fewer tokens than two rounds of warps deals the heads over more warps,
+// in whole batches of loads.
+void plan_runs(RopeParams& p, int heads, int D, int elem) {
+  const int batch = 32 / (D / 8) * (elem == 2 ? 4 : 2);
+  const long want = 148L * 24 * 2;
   const long runs = std::min<long>((heads + batch - 1) / batch, std::max<long>(1, want / p.T));
   p.run = static_cast<int>((heads + runs - 1) / runs + batch - 1) / batch * batch;
   p.runs = (heads + p.run - 1) / p.run;
@@ -486,10 +508,13 @@ void dispatch(const at::Tensor& q, bool interleaved, F&& f) {
 
 }  // namespace
 
-std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& q_weight,
+std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q_in, const c10::optional<at::Tensor>& k_in,
+                                    const c10::optional<at::Tensor>& q_weight,
                                     const c10::optional<at::Tensor>& k_weight,
                                     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& freqs,
                                     const std::vector<int64_t>& pairs, bool interleaved, bool inverse, double eps) {
+  const at::Tensor q = fit(q_in);
+  const at::Tensor k = k_in.has_value() ? fit(*k_in) : q.narrow(1, 0, 0);
   RopeParams p = make_params(q, k, positions, freqs, pairs, inverse, eps);
   TORCH_CHECK(q_weight.has_value() == k_weight.has_value(), "q_weight and k_weight come together");
   const void *qw = nullptr, *kw = nullptr;
@@ -500,11 +525,11 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const at::Tensor& k, co
     TORCH_CHECK(kb == p.w_bf16, "q_weight and k_weight must have one type");
   }
   c10::cuda::CUDAGuard guard(q.get_device());
-  auto q_out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
-  auto k_out = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
+  auto q_out = empty_cuda(q.sizes(), q.scalar_type(), q);
+  auto k_out = empty_cuda(k.sizes(), k.scalar_type(), k);
   const int heads = p.Hq + p.Hk, D = static_cast<int>(q.size(2));
   if (p.T == 0 || heads == 0) return {q_out, k_out};
-  plan_runs(p, heads, D);
+  plan_runs(p, heads, D, static_cast<int>(q.element_size()));
   const long blocks = (p.T * p.runs + kThreads / 32 - 1) / (kThreads / 32);
   TORCH_CHECK(blocks < (1L << 31), "too many tokens");
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
@@ -525,11 +550,12 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const at::Tensor& k, co
   return {q_out, k_out};
 }
 
-std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& q_weight,
                                          const at::Tensor& k_weight, const c10::optional<at::Tensor>& positions,
                                          const c10::optional<at::Tensor>& freqs, const std::vector<int64_t>& pairs,
-                                         bool interleaved, const at::Tensor& dq_out, const at::Tensor& dk_out,
+                                         bool interleaved, const at::Tensor& dq_in, const at::Tensor& dk_in,
                                          double eps) {
+  const at::Tensor q = fit(q_in), k = fit(k_in), dq_out = fit(dq_in), dk_out = fit(dk_in);
   RopeParams p = make_params(q, k, positions, freqs, pairs, false, eps);
   bool kb = false;
   const void* qw = check_weight(q_weight, q, "q_weight", p.w_bf16);
@@ -540,15 +566,15 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q, const at::Tensor& 
   TORCH_CHECK(dq_out.size(1) == q.size(1) && dk_out.size(1) == k.size(1), "dq and dk must have the heads of q and k");
   p.dq_tok = dq_out.stride(0), p.dq_head = dq_out.stride(1), p.dk_tok = dk_out.stride(0), p.dk_head = dk_out.stride(1);
   c10::cuda::CUDAGuard guard(q.get_device());
-  auto dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
-  auto dk = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
+  auto dq = empty_cuda(q.sizes(), q.scalar_type(), q);
+  auto dk = empty_cuda(k.sizes(), k.scalar_type(), k);
   const int heads = p.Hq + p.Hk, D = static_cast<int>(q.size(2));
   if (p.T == 0 || heads == 0) {
     auto zero = at::zeros({2, D}, q.options().dtype(at::kFloat));
     return {dq, dk, zero[0], zero[1]};
   }
-  auto dw = at::empty({2, D}, q.options().dtype(at::kFloat));
-  plan_runs(p, heads, D);
+  auto dqw = empty_cuda({D}, at::kFloat, q), dkw = empty_cuda({D}, at::kFloat, q);
+  plan_runs(p, heads, D, static_cast<int>(q.element_size()));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
   dispatch(q, interleaved, [&](auto* type, auto dim, auto inter) {
     using T = std::remove_pointer_t<decltype(type)>;
@@ -557,19 +583,19 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q, const at::Tensor& 
     auto kernel = qk_norm_rope_bwd_kernel<T, kD, kInter>;
     const long blocks = (p.T * p.runs + kThreads / 32 - 1) / (kThreads / 32);
     const int grid = static_cast<int>(std::min<long>(blocks, resident_blocks(kernel)));
-    auto partial = at::empty({grid, 2 * D}, dw.options());
+    auto partial = empty_cuda({grid, 2 * kD}, at::kFloat, q);
     kernel<<<grid, kThreads, 0, stream>>>(
         reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
         reinterpret_cast<const T*>(dq_out.data_ptr()), reinterpret_cast<const T*>(dk_out.data_ptr()),
         reinterpret_cast<T*>(dq.data_ptr()), reinterpret_cast<T*>(dk.data_ptr()), partial.data_ptr<float>(), p);
     note_launch();
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    sum_partials_kernel<<<2 * kD / 32, dim3(32, 32), 0, stream>>>(partial.data_ptr<float>(), grid, 2 * kD,
-                                                                  dw.data_ptr<float>());
+    sum_partials_kernel<<<2 * kD / 32, dim3(32, 32), 0, stream>>>(partial.data_ptr<float>(), grid, kD,
+                                                                  dqw.data_ptr<float>(), dkw.data_ptr<float>());
     note_launch();
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
-  return {dq, dk, dw[0], dw[1]};
+  return {dq, dk, dqw, dkw};
 }
 
 }  // namespace h3

@@ -6,10 +6,11 @@
 
 namespace h3 {
 
-// q [T, Hq, D], k [T, Hk, D] (bf16 or fp32; Hk may be 0) -> rotated {q, k}, contiguous.
+// q [T, Hq, D], k [T, Hk, D] (bf16 or fp32; k may be absent) -> rotated {q, k}, contiguous.
 // With weights ([D], bf16 or fp32) every head is RMS-normalised and scaled first.
 // positions [T, A] fp32 and freqs [sum(pairs)] fp32 may be absent (no rotation).
-std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& q_weight,
+std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const c10::optional<at::Tensor>& k,
+                                    const c10::optional<at::Tensor>& q_weight,
                                     const c10::optional<at::Tensor>& k_weight,
                                     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& freqs,
                                     const std::vector<int64_t>& pairs, bool interleaved, bool inverse, double eps);

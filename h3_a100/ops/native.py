@@ -43,20 +43,6 @@ STATUS_NAMES = {1: "timeout waiting for a TMA stage", 2: "timeout waiting for a 
                 7: "out-of-bounds access caught by the bounds-checked build"}
 
 
-def _heads16(t: torch.Tensor) -> torch.Tensor:
-    """``t [tokens, heads, D]`` itself if the kernels can read its layout, else a contiguous copy.
-
-    They need unit stride within a head and every head on a 16-byte boundary
-    (a vector load, a TMA row); an expanded (zero-stride) dimension has no such layout.
-    """
-    unit = 16 // t.element_size()
-    if t.dim() != 3 or t.numel() == 0:
-        return t
-    fits = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-        t.shape[d] == 1 or (t.stride(d) > 0 and t.stride(d) % unit == 0) for d in (0, 1))
-    return t if fits else t.contiguous()
-
-
 def _num_sms(device: torch.device) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
@@ -210,31 +196,30 @@ class NativeKernels:
         return self.C.attention_bwd(qkv, o, lse, do, int(heads), int(head_dim), self.status, self.limit_ns)
 
     # ------------------------------------------------------------ packed sequences
+    # Tensors whose layout the kernels cannot read (a head off a 16-byte
+    # boundary, an expanded dimension) are copied first.
     @staticmethod
     def _rope_args(rope: AxisRope | None):
         if rope is None:
             return None, None, [], True
-        return rope.positions, rope.freqs, list(rope.pairs), rope.interleaved
+        return rope.positions, rope.freqs, rope.pairs, rope.interleaved
 
     def rope_axes(self, q, k, rope: AxisRope, inverse: bool = False):
         """Rotate every head of ``q`` and ``k`` (``k`` may be None); ``inverse`` turns gradients back."""
         pos, freqs, pairs, inter = self._rope_args(rope)
-        both = self.C.qk_rope_fwd(_heads16(q), q[:, :0] if k is None else _heads16(k), None, None, pos, freqs, pairs,
-                                  inter, bool(inverse), 0.0)
+        both = self.C.qk_rope_fwd(q, k, None, None, pos, freqs, pairs, inter, bool(inverse), 0.0)
         return both[0], None if k is None else both[1]
 
     def qk_norm_rope(self, q, k, q_weight, k_weight, rope: AxisRope | None = None, eps=1e-6):
         """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``), then the rotation."""
         pos, freqs, pairs, inter = self._rope_args(rope)
-        both = self.C.qk_rope_fwd(_heads16(q), _heads16(k), q_weight, k_weight, pos, freqs, pairs, inter, False,
-                                  float(eps))
+        both = self.C.qk_rope_fwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, False, float(eps))
         return both[0], both[1]
 
     def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6):
         """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32."""
         pos, freqs, pairs, inter = self._rope_args(rope)
-        return tuple(self.C.qk_norm_rope_bwd(_heads16(q), _heads16(k), q_weight, k_weight, pos, freqs, pairs, inter,
-                                             _heads16(dq), _heads16(dk), float(eps)))
+        return tuple(self.C.qk_norm_rope_bwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, dq, dk, float(eps)))
 
     def packed_plan(self, q_lens, k_lens=None, *, heads, kv_heads, head_dim, causal=False) -> PackedPlan:
         """Work lists of a packed batch, uploaded once; every layer's forward and backward uses them."""
@@ -256,8 +241,7 @@ class NativeKernels:
         bf16, head dim 64 or 128; see ``TorchKernels.attention_packed_fwd``.
         """
         blob, meta, scale = self._packed_args(plan, scale)
-        o, lse = self.C.attention_packed_fwd(_heads16(q), _heads16(k), _heads16(v), blob, meta, scale, self.status,
-                                             self.limit_ns)
+        o, lse = self.C.attention_packed_fwd(q, k, v, blob, meta, scale, self.status, self.limit_ns)
         return o, lse
 
     def attention_packed_bwd(self, q, k, v, o, lse, do, plan: PackedPlan, scale=None, out=None):
@@ -267,8 +251,7 @@ class NativeKernels:
         order: the same inputs give the same bits.
         """
         blob, meta, scale = self._packed_args(plan, scale)
-        return tuple(self.C.attention_packed_bwd(_heads16(q), _heads16(k), _heads16(v), _heads16(o), lse, _heads16(do),
-                                                 blob, meta, scale, self.status, self.limit_ns,
+        return tuple(self.C.attention_packed_bwd(q, k, v, o, lse, do, blob, meta, scale, self.status, self.limit_ns,
                                                  [] if out is None else list(out)))
 
     # ------------------------------------------------------------ small projections
