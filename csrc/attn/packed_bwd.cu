@@ -85,23 +85,21 @@ __device__ __forceinline__ void issue_accum(uint32_t d_tmem, uint32_t a_tmem, ui
 template <int COLS>
 __device__ __forceinline__ void store_row(uint32_t taddr, bool any, float scale, __nv_bfloat16* out, long off, bool live,
                                           long extent, const KernelStatus& st) {
+  const bool aligned32 = (reinterpret_cast<uintptr_t>(out + off) & 31u) == 0;
+#pragma unroll 1
+  for (int c0 = 0; c0 < COLS; c0 += 32) {      // 32 columns a wait (the register budget)
+    uint32_t r[2][16];
+    tmem_ld16(taddr + c0, r[0]);
+    tmem_ld16(taddr + c0 + 16, r[1]);
+    tmem_ld_wait();
 #pragma unroll
-  for (int c = 0; c < COLS / 16; ++c) {
-    uint32_t r[16];
-    if (any) {
-      tmem_ld16(taddr + c * 16, r);
-      tmem_ld_wait();
+    for (int c = 0; c < 2; ++c) {
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = any ? __uint_as_float(r[c][k]) * scale : 0.f;
+      const long first = off + c0 + c * 16;
+      if (live && H3_IN_BOUNDS(first, first + 15, extent, st)) store16_bf16(out + first, v, aligned32);
     }
-    float v[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = any ? __uint_as_float(r[k]) * scale : 0.f;
-    const long first = off + c * 16;
-    if (!live || !H3_IN_BOUNDS(first, first + 15, extent, st)) continue;
-    uint4* dst = reinterpret_cast<uint4*>(out + first);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      dst[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                          pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
   }
 }
 
@@ -181,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   b.dp_full = nb + 6, b.ds_full = nb + 8, b.dq_full = nb + 10, b.drain = nb + 11;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const Slice own(p.items, p.begin);
   const int warp = warp_id();
   const uint64_t limit = p.status.limit_ns;
   if (threadIdx.x == 0) {
@@ -203,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int begin = p.begin[blockIdx.x], end = p.begin[blockIdx.x + 1];
+  const int begin = own.begin, end = own.end;
   if (warp < 4) {
     setmaxnreg_dec<kRegsLow>();
     if (warp == 0 && elect_one()) {
@@ -213,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int q_used = 0, do_used = 0;
       bool ok = true;
       for (int i = begin; i < end && ok; ++i) {
-        const PackedItem it = load_item(p.items + i);
+        const PackedItem it = own.item(p, i);
         int tail;
         const int n = key_tiles(it, tail);
         if (n == 0) continue;
@@ -264,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t q_desc = k_major(sQ), k_desc = k_major(rk.base);
       for (int i = begin; i < end && ok; ++i) {
         int tail;
-        const int n = key_tiles(load_item(p.items + i), tail);
+        const int n = key_tiles(own.item(p, i), tail);
         for (int j = 0; j < n; ++j, ++st, k.next()) {
           ok = mbar_wait(&rk.full[k.slot], k.phase, limit, abort_flag) &&
                (j > 0 || mbar_wait(b.q_full, items & 1u, limit, abort_flag)) &&
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t do_desc = k_major(sDO), v_desc = k_major(rv.base), k_desc = mn_major(rk.base);
       for (int i = begin; i < end && ok; ++i) {
         int tail;
-        const int n = key_tiles(load_item(p.items + i), tail);
+        const int n = key_tiles(own.item(p, i), tail);
         if (n == 0) continue;
         // dP runs a step ahead in the other buffer: the dS that was there has been used by the product before.
         auto grads = [&](int j) {
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int nk = 0;
       uint32_t parity = 0;
       for (int i = begin; i < end; ++i) {
-        const PackedItem it = load_item(p.items + i);
+        const PackedItem it = own.item(p, i);
         int tail;
         const int n = key_tiles(it, tail);
         if (tail != 0 && !clean_tile<C::kChunks, C::kTile>(rk, nk + n - 1, tail, parity, limit, abort_flag)) {
@@ -347,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int st = 0, items = 0;
   bool ok = true;
   for (int i = begin; i < end; ++i) {
-    const PackedItem it = load_item(p.items + i);
+    const PackedItem it = own.item(p, i);
     int tail;
     const int n = key_tiles(it, tail);
     const bool live = row < it.nq * p.G;
@@ -466,6 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   b.ds_full = nb + 6, b.acc_full = nb + 8, b.row_full = nb + 9, b.drain = nb + 11;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const Slice own(p.items, p.begin);
   const int warp = warp_id();
   const uint64_t limit = p.status.limit_ns;
   const int rows_full = p.bt * p.G;      // rows of a whole query tile
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int begin = p.begin[blockIdx.x], end = p.begin[blockIdx.x + 1];
+  const int begin = own.begin, end = own.end;
   // Query tiles of an item and live rows of the last one.
   auto query_tiles = [&](const PackedItem& it, int& last_rows) {
     const int n = (it.nq + p.bt - 1) / p.bt;
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int used = 0;
       bool ok = true;
       for (int i = begin; i < end && ok; ++i) {
-        const PackedItem it = load_item(p.items + i);
+        const PackedItem it = own.item(p, i);
         int last_rows, slot;
         const int n = query_tiles(it, last_rows);
         if (n == 0) continue;
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t items = 0;
       for (int i = begin; i < end && ok; ++i) {
         int last_rows;
-        const int n = query_tiles(load_item(p.items + i), last_rows);
+        const int n = query_tiles(own.item(p, i), last_rows);
         if (n == 0) continue;
         auto scores = [&]() {
           if (!mbar_wait(&rq.full[q_ahead.slot], q_ahead.phase, limit, abort_flag) ||
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t pq = 0, pd = 0;
       bool ok = true;
       for (int i = begin; i < end && ok; ++i) {
-        const PackedItem it = load_item(p.items + i);
+        const PackedItem it = own.item(p, i);
         int last_rows;
         const int n = query_tiles(it, last_rows);
         for (int j = 0; j < n; ++j, ++st) {
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int st = 0, items = 0;
   bool ok = true;
   for (int i = begin; i < end; ++i) {
-    const PackedItem it = load_item(p.items + i);
+    const PackedItem it = own.item(p, i);
     int last_rows;
     const int n = query_tiles(it, last_rows);
     for (int j = 0; j < n; ++j, ++st) {

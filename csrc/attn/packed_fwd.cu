@@ -98,7 +98,7 @@ __device__ __forceinline__ TileWork tile_work(const PackedItem& it, int bt) {
 template <int D>
 __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                           const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kK>& rk,
-                                          const Ring<Fwd<D>::kV>& rv, const Bars& b, volatile int* abort_flag) {
+                                          const Ring<Fwd<D>::kV>& rv, const Bars& b, volatile int* abort_flag, const Slice& own) {
   using C = Fwd<D>;
   const uint64_t limit = p.status.limit_ns;
   const uint32_t q_bytes = static_cast<uint32_t>(p.bt * p.G) * 128u * C::kChunks;
@@ -106,23 +106,20 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorM
   Feed<C::kV> fv;
   int q_used[2] = {0, 0};
   bool ok = true;
-  const int end = p.begin[blockIdx.x + 1];
-  for (int i = p.begin[blockIdx.x]; i < end && ok; ++i) {
-    const PackedItem it = load_item(p.items + i);
+  for (int i = own.begin; i < own.end && ok; ++i) {
+    const PackedItem it = own.item(p, i);
     const TileWork w = tile_work(it, p.bt);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (w.n(t) == 0 || (w.solo && t == 1) || !ok) continue;
-      if (!mbar_wait(&b.q_empty[t], (q_used[t] & 1) ^ 1u, limit, abort_flag)) {
-        ok = false;
-        break;
-      }
+    auto load_q = [&](int t) {
+      if (w.n(t) == 0 || (w.solo && t == 1)) return true;
+      if (!mbar_wait(&b.q_empty[t], (q_used[t] & 1) ^ 1u, limit, abort_flag)) return false;
       ++q_used[t];
       mbar_arrive_expect_tx(&b.q_full[t], q_bytes);
 #pragma unroll
       for (int c = 0; c < C::kChunks; ++c)
         tma_load_4d(sQ + t * C::kTile + c * kChunkBytes, &tq, &b.q_full[t], c * 64, 0, it.head, it.q0 + t * p.bt);
-    }
+      return true;
+    };
+    ok = load_q(0);
     for (int kt = 0; kt < w.most && ok; ++kt) {
       int slot;
       uint64_t* full = fk.next(rk, false, C::kTile, limit, abort_flag, slot);
@@ -131,6 +128,8 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorM
 #pragma unroll
       for (int c = 0; c < C::kChunks; ++c)
         tma_load_3d(rk.base + slot * C::kTile + c * kChunkBytes, &tk, full, c * 64, it.head, it.k0 + kt * 128);
+      if (kt == 0) ok = load_q(1);      // after what the first product needs
+      if (!ok) break;
       full = fv.next(rv, w.tail != 0 && kt + 1 == w.most, C::kTile, limit, abort_flag, slot);
       ok = full != nullptr;
       if (!ok) break;
@@ -153,7 +152,7 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorM
 // All scores, in the order (key tile, warpgroup).
 template <int D>
 __device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kK>& rk, const Bars& b,
-                                           volatile int* abort_flag, uint32_t tmem) {
+                                           volatile int* abort_flag, const Slice& own, uint32_t tmem) {
   using C = Fwd<D>;
   constexpr uint32_t kIdesc = umma_idesc_bf16(128, 128, false, false);
   const uint64_t limit = p.status.limit_ns;
@@ -161,9 +160,8 @@ __device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ
   Cursor<C::kK> k;
   uint32_t q_used0 = 0, q_used1 = 0, issued = 0;
   bool ok = true;
-  const int end = p.begin[blockIdx.x + 1];
-  for (int i = p.begin[blockIdx.x]; i < end && ok; ++i) {
-    const TileWork w = tile_work(load_item(p.items + i), p.bt);
+  for (int i = own.begin; i < own.end && ok; ++i) {
+    const TileWork w = tile_work(own.item(p, i), p.bt);
     for (int kt = 0; kt < w.most && ok; ++kt, k.next()) {
       ok = mbar_wait(&rk.full[k.slot], k.phase, limit, abort_flag);
 #pragma unroll
@@ -200,7 +198,7 @@ __device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ
 // All products with V, in the same order.
 template <int D>
 __device__ __forceinline__ void value_warp(const PackedFwdParams& p, const Ring<Fwd<D>::kV>& rv, const Bars& b,
-                                           volatile int* abort_flag, uint32_t tmem) {
+                                           volatile int* abort_flag, const Slice& own, uint32_t tmem) {
   using C = Fwd<D>;
   constexpr uint32_t kIdesc = umma_idesc_bf16(128, D, false, true);
   const uint64_t limit = p.status.limit_ns;
@@ -208,9 +206,8 @@ __device__ __forceinline__ void value_warp(const PackedFwdParams& p, const Ring<
   Cursor<C::kV> v;
   uint32_t steps0 = 0, steps1 = 0;
   bool ok = true;
-  const int end = p.begin[blockIdx.x + 1];
-  for (int i = p.begin[blockIdx.x]; i < end && ok; ++i) {
-    const TileWork w = tile_work(load_item(p.items + i), p.bt);
+  for (int i = own.begin; i < own.end && ok; ++i) {
+    const TileWork w = tile_work(own.item(p, i), p.bt);
     for (int kt = 0; kt < w.most && ok; ++kt, v.next()) {
       ok = mbar_wait(&rv.full[v.slot], v.phase, limit, abort_flag);
 #pragma unroll
@@ -238,13 +235,12 @@ __device__ __forceinline__ void value_warp(const PackedFwdParams& p, const Ring<
 // Zeroes the rows past the sequence in the last V tile of each item that has such rows.
 template <int D>
 __device__ __forceinline__ void clean_warp(const PackedFwdParams& p, const Ring<Fwd<D>::kV>& rv,
-                                           volatile int* abort_flag) {
+                                           volatile int* abort_flag, const Slice& own) {
   using C = Fwd<D>;
   int base = 0;
   uint32_t parity = 0;
-  const int end = p.begin[blockIdx.x + 1];
-  for (int i = p.begin[blockIdx.x]; i < end; ++i) {
-    const TileWork w = tile_work(load_item(p.items + i), p.bt);
+  for (int i = own.begin; i < own.end; ++i) {
+    const TileWork w = tile_work(own.item(p, i), p.bt);
     if (w.tail != 0 &&
         !clean_tile<C::kChunks, C::kTile>(rv, base + w.most - 1, w.tail, parity, p.status.limit_ns, abort_flag)) {
       if (lane_id() == 0) {
@@ -292,7 +288,7 @@ __device__ __forceinline__ float row_exp(uint32_t (&r)[4][32], float scale, floa
 }
 
 template <int D>
-__device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Bars& b, volatile int* abort_flag,
+__device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Bars& b, volatile int* abort_flag, const Slice& own,
                                               float2* exchange, uint32_t tmem, int t) {
   const uint64_t limit = p.status.limit_ns;
   const int row = (warp_id() & 3) * 32 + lane_id();
@@ -301,9 +297,8 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
   const int tok = row / p.G, g = row - tok * p.G;   // token of the tile and head of the group of this row
   int steps = 0;          // this warpgroup's key tiles so far
   bool ok = true;
-  const int end = p.begin[blockIdx.x + 1];
-  for (int i = p.begin[blockIdx.x]; i < end; ++i) {
-    const PackedItem it = load_item(p.items + i);
+  for (int i = own.begin; i < own.end; ++i) {
+    const PackedItem it = own.item(p, i);
     const TileWork w = tile_work(it, p.bt);
     const int first = w.solo ? 0 : t * p.bt, n_kv = w.n(t);
     const bool both = w.solo && w.n1 > 0;      // one query tile, both warpgroups on it
@@ -390,39 +385,39 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
     const bool part = it.slot >= 0;
     const long part_row = (static_cast<long>(it.slot) + (w.solo ? 0 : t * it.pad)) * p.part_rows + row;
     const long o_off = part ? part_row * D : (q * p.Hq + head) * D;
-    constexpr int kPieces = D / 16;
-    const int c0 = both && t == 1 ? kPieces / 2 : 0, c1 = both && t == 0 ? kPieces / 2 : kPieces;
-#pragma unroll 2
-    for (int c = c0; c < c1; ++c) {
-      float v[16];
-#pragma unroll
-      for (int k = 0; k < 16; ++k) v[k] = 0.f;
-      if (n_kv > 0) {
-        uint32_t r[16];
-        tmem_ld16(tO + t * 128 + c * 16, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = some ? __uint_as_float(r[k]) * scale_own : 0.f;
-      }
+    // 32 TMEM columns a wait (the register budget): 32 of this row's O_t, or 16 of each accumulator.
+    const int first_col = both ? t * (D / 2) : 0, cols = both ? D / 2 : D, step = both ? 16 : 32;
+#pragma unroll 1
+    for (int c = 0; c < cols; c += step) {
+      const int col = first_col + c;
+      uint32_t r[2][16];      // without a key tile (`some` is false then): whatever is there
+      tmem_ld16(tO + t * 128 + col, r[0]);
+      tmem_ld16(both ? tO + (t ^ 1) * 128 + col : tO + t * 128 + col + 16, r[1]);
+      tmem_ld_wait();
       if (both) {
-        uint32_t r[16];
-        tmem_ld16(tO + (t ^ 1) * 128 + c * 16, r);
-        tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = some ? fmaf(__uint_as_float(r[k]), scale_other, v[k]) : 0.f;
+        for (int k = 0; k < 16; ++k)
+          r[0][k] = __float_as_uint(__uint_as_float(r[0][k]) * scale_own + __uint_as_float(r[1][k]) * scale_other);
       }
-      const long at = o_off + c * 16;
-      if (!live || !H3_IN_BOUNDS(at, at + 15, part ? p.part_extent : p.o_extent, p.status)) continue;
-      if (part) {
-        float4* dst = reinterpret_cast<float4*>(p.part_o + at);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dst[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-      } else {
-        uint4* dst = reinterpret_cast<uint4*>(p.o + at);
+      for (int h = 0; h < 2; ++h) {
+        if (h > 0 && both) continue;
+        float v[16];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          dst[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                              pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+        for (int k = 0; k < 16; ++k) v[k] = some ? __uint_as_float(r[h][k]) * (both ? 1.f : scale_own) : 0.f;
+        const long at = o_off + col + h * 16;
+        if (!live || !H3_IN_BOUNDS(at, at + 15, part ? p.part_extent : p.o_extent, p.status)) continue;
+        if (part) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(v[8 * k + e]);
+            store32(p.part_o + at + 8 * k, u);
+          }
+        } else {
+          store16_bf16(p.o + at, v, true);      // o is contiguous, allocated here
+        }
       }
     }
     const long lse_off = static_cast<long>(head) * p.Tq + q;
@@ -466,6 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13 + rk.kBarriers + rv.kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id();
+  const Slice own(p.items, p.begin);
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&b.q_full[t], 1);
@@ -496,13 +492,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     setmaxnreg_dec<kRegsLow>();
     if (warp == 0) {
-      if (elect_one()) load_warp<D>(tq, tk, tv, p, sQ, rk, rv, b, abort_flag);
+      if (elect_one()) load_warp<D>(tq, tk, tv, p, sQ, rk, rv, b, abort_flag, own);
     } else if (warp == 1) {
-      if (elect_one()) score_warp<D>(p, sQ, rk, b, abort_flag, tmem);
+      if (elect_one()) score_warp<D>(p, sQ, rk, b, abort_flag, own, tmem);
     } else if (warp == 2) {
-      clean_warp<D>(p, rv, abort_flag);
+      clean_warp<D>(p, rv, abort_flag, own);
     } else {
-      if (elect_one()) value_warp<D>(p, rv, b, abort_flag, tmem);
+      if (elect_one()) value_warp<D>(p, rv, b, abort_flag, own, tmem);
     }
     __syncwarp();
     tc_fence_before();
@@ -514,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   setmaxnreg_inc<kRegsHigh>();
-  softmax_warps<D>(p, b, abort_flag, exchange, tmem, (warp - 4) >> 2);
+  softmax_warps<D>(p, b, abort_flag, own, exchange, tmem, (warp - 4) >> 2);
   __syncwarp();
   tc_fence_before();
   named_bar_sync(1, kThreads);
@@ -528,31 +524,40 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const PackedJoin* __re
   const PackedJoin jn = list[blockIdx.x];
   const int rows = jn.nq * p.G, lane = lane_id();
   for (int row = blockIdx.y * 4 + warp_id(); row < rows; row += gridDim.y * 4) {
-    const float* lses = p.part_lse + static_cast<long>(jn.slot0) * p.part_rows + row;
-    float m = -INFINITY;
-    for (int i = lane; i < jn.parts; i += 32) m = fmaxf(m, lses[static_cast<long>(i) * p.part_rows]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    float acc[kPer], sum = 0.f;
+    const long first = static_cast<long>(jn.slot0) * p.part_rows + row;
+    float m = -INFINITY, sum = 0.f, acc[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < jn.parts; ++i) {
-      const long r = (static_cast<long>(jn.slot0) + i) * p.part_rows + row;
-      const float wgt = ex2(lses[static_cast<long>(i) * p.part_rows] - base);
-      const float* src = p.part_o + r * D + lane * kPer;
-      float v[kPer];
-      if (kPer == 4) {
-        const float4 u = *reinterpret_cast<const float4*>(src);
-        v[0] = u.x, v[1] = u.y, v[kPer - 2] = u.z, v[kPer - 1] = u.w;
-      } else {
-        const float2 u = *reinterpret_cast<const float2*>(src);
-        v[0] = u.x, v[1] = u.y;
-      }
-      sum += wgt;
+    // Four parts' loads at a time: most rows have no more, and wait for memory once.
+    for (int i0 = 0; i0 < jn.parts; i0 += 4) {
+      float lse[4], v[4][kPer], top = m;
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[k] = fmaf(wgt, v[k], acc[k]);
+      for (int i = 0; i < 4; ++i) {
+        const bool have = i0 + i < jn.parts;
+        const long r = first + static_cast<long>(i0 + i) * p.part_rows;
+        lse[i] = have ? p.part_lse[r] : -INFINITY;
+        if (kPer == 4) {
+          const float4 u = have ? *reinterpret_cast<const float4*>(p.part_o + r * D + lane * kPer) : float4{};
+          v[i][0] = u.x, v[i][1] = u.y, v[i][kPer - 2] = u.z, v[i][kPer - 1] = u.w;
+        } else {
+          const float2 u = have ? *reinterpret_cast<const float2*>(p.part_o + r * D + lane * kPer) : float2{};
+          v[i][0] = u.x, v[i][1] = u.y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, lse[i]);
+      const float base = top == -INFINITY ? 0.f : top, old = ex2(m - base);
+      m = top;
+      sum *= old;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] *= old;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float weight = ex2(lse[i] - base);
+        sum += weight;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(weight, v[i][k], acc[k]);
+      }
     }
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     const int tok = row / p.G, head = jn.head * p.G + row - tok * p.G;

@@ -84,6 +84,27 @@ __device__ __forceinline__ void named_bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// 32 bytes in one store (a whole sector; as two 16-byte stores a warp's rows
+// make twice the write transactions).  `p` on a 32-byte boundary.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 16 values as bf16 at `p`; 16-byte stores where the row is not on a 32-byte boundary.
+__device__ __forceinline__ void store16_bf16(__nv_bfloat16* p, const float (&v)[16], bool aligned32) {
+  uint32_t u[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) u[k] = pack_bf16x2(v[2 * k], v[2 * k + 1]);
+  if (aligned32) {
+    store32(p, u);
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+  }
+}
+
 // One arrival for the whole warp (32 on one address would be taken one by one).
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();
@@ -131,6 +152,21 @@ __device__ __forceinline__ PackedItem load_item(const PackedItem* p) {
   it.q0 = a.x, it.nq = a.y, it.k0 = a.z, it.nk = a.w, it.diag = b.x, it.head = b.y, it.slot = b.z, it.pad = b.w;
   return it;
 }
+
+// This block's part of the work list; its first item is read at once, beside the kernel's set-up.
+struct Slice {
+  int begin, end;
+  PackedItem first;
+  __device__ __forceinline__ Slice(const PackedItem* items, const int* starts) {
+    begin = __ldg(starts + blockIdx.x);
+    end = __ldg(starts + blockIdx.x + 1);
+    first = load_item(items + begin);      // a block is launched for one item at least
+  }
+  template <typename P>
+  __device__ __forceinline__ PackedItem item(const P& p, int i) const {
+    return i == begin ? first : load_item(p.items + i);
+  }
+};
 
 // A ring of tiles.  A tile whose last rows must be zeroed arrives on tail[slot];
 // the cleaning warp then makes the arrival on full[slot].
