@@ -385,17 +385,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(&b.dp_full[st & 1], (st >> 1) & 1, limit, abort_flag));
       if (!ok) break;
       tc_fence_after();
-      uint32_t packed[2][16];
+      uint32_t packed[2][16], dp[2][32];
+      tmem_ld32(tP, dp[0]);
+      tmem_ld32(tP + 32, dp[1]);
+      tmem_ld_wait();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t dp[32];
-        tmem_ld32(tP + c * 32, dp);
-        tmem_ld_wait();
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           float x, y;
-          unpack2(mul2(pr[c][k], add2(pack2(__uint_as_float(dp[2 * k]), __uint_as_float(dp[2 * k + 1])), neg_delta)), x,
-                  y);
+          unpack2(mul2(pr[c][k], add2(pack2(__uint_as_float(dp[c][2 * k]), __uint_as_float(dp[c][2 * k + 1])), neg_delta)),
+                  x, y);
           if (cut) {   // a select, not a product: what a masked place holds may be NaN
             x = c * 32 + 2 * k < valid ? x : 0.f;
             y = c * 32 + 2 * k + 1 < valid ? y : 0.f;
@@ -428,6 +428,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- dk, dv
+// Whether P^T is handed over before dS^T.  At D = 128 the products set the pace
+// and dV fills the wait for dS (16,384 x 8 heads: 1,525 -> 1,437 us); at D = 64 the
+// softmax warps do and a second hand-over costs them (1,212 -> 1,352 us).
+template <int D>
+constexpr bool kEarlyP = D == 128;
+
 // Zeros in the first `hidden` of a row's 64 values.
 __device__ __forceinline__ void hide(uint64_t (&v)[2][16], int hidden) {
 #pragma unroll
@@ -441,7 +447,7 @@ __device__ __forceinline__ void hide(uint64_t (&v)[2][16], int hidden) {
 }
 
 struct DkvBars {
-  uint64_t *k_full, *v_full, *kv_empty, *s_full, *s_read, *dp_full, *ds_full, *acc_full, *row_full, *drain;
+  uint64_t *k_full, *v_full, *kv_empty, *s_full, *s_read, *dp_full, *ds_full, *acc_full, *row_full, *p_full, *drain;
 };
 
 template <int D>
@@ -462,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   DkvBars b;
   uint64_t* nb = bars + rq.kBarriers + rd.kBarriers;
   b.k_full = nb, b.v_full = nb + 1, b.kv_empty = nb + 2, b.s_full = nb + 3, b.s_read = nb + 4, b.dp_full = nb + 5;
-  b.ds_full = nb + 6, b.acc_full = nb + 8, b.row_full = nb + 9, b.drain = nb + 11;
+  b.ds_full = nb + 6, b.acc_full = nb + 8, b.row_full = nb + 9, b.p_full = nb + 11, b.drain = nb + 12;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nb + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const Slice own(p.items, p.begin);
@@ -472,8 +478,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     rq.init();
     rd.init();
-    for (int i = 0; i < 13; ++i)
-      mbar_init(nb + i, nb + i == b.s_read || nb + i == b.ds_full || nb + i == b.ds_full + 1 ? 8 : 1);
+    for (int i = 0; i < 13; ++i) {
+      uint64_t* at = nb + i;
+      mbar_init(at, at == b.s_read || at == b.ds_full || at == b.ds_full + 1 || at == b.p_full ? 8 : 1);
+    }
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tq);
@@ -555,8 +563,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 1 && elect_one()) {
       // One thread for all products, in the order dV dK dP' S'' of steps j, j, j + 1,
-      // j + 2: S'' then runs while the softmax warps turn dP' into dS', which
-      // is the one stretch where no other product is ready.
+      // j + 2: S'' runs while the softmax warps store P' and dV' while they turn
+      // dP' into dS', the one stretch where nothing else is ready.
       Cursor<C::kLong> q, q_ahead;      // tiles of the next dK and of the next S
       Cursor<C::kShort> d, d_ahead;     // tiles of the next dV and of the next dP
       uint32_t st = 0, scored = 0;      // steps used up, steps scored
@@ -590,12 +598,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = mbar_wait(b.k_full, items & 1u, limit, abort_flag) && scores() &&
              mbar_wait(b.v_full, items & 1u, limit, abort_flag) && grads() && (n == 1 || scores());
         for (int j = 0; j < n && ok; ++j, ++st, q.next(), d.next()) {
-          ok = mbar_wait(&b.ds_full[st & 1u], (st >> 1) & 1u, limit, abort_flag);
+          // P^T of the two warpgroups at columns 384 and 448, dS^T at 416 and 480.
+          ok = kEarlyP<D> ? mbar_wait(b.p_full, st & 1u, limit, abort_flag)
+                          : mbar_wait(&b.ds_full[st & 1u], (st >> 1) & 1u, limit, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          // P^T of the two warpgroups at columns 384 and 448, dS^T at 416 and 480.
           issue_accum<D>(tmem, tmem + 384, 64, dm_desc + static_cast<uint64_t>(d.slot * C::kTile16), j == 0);
           umma_commit(&rd.empty[d.slot]);
+          if (kEarlyP<D>) ok = mbar_wait(&b.ds_full[st & 1u], (st >> 1) & 1u, limit, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
           issue_accum<D>(tmem + 128, tmem + 416, 64, qm_desc + static_cast<uint64_t>(q.slot * C::kTile16), j == 0);
           umma_commit(&rq.empty[q.slot]);
           // The next dP overwrites P^T and dS^T: one thread's products run in order.
@@ -715,9 +727,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(tP + 32, dp[1]);
       tmem_ld_wait();
       // This warpgroup's dP columns are read: P^T goes over the first half of them, dS^T over the second.
+      tmem_st16(tP, pp[0]);
+      tmem_st16(tP + 16, pp[1]);
+      if (kEarlyP<D>) {
+        tmem_st_wait();
+        tc_fence_before();
+        warp_arrive(b.p_full);
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        tmem_st16(tP + c * 16, pp[c]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const ulonglong2 neg_delta = *reinterpret_cast<const ulonglong2*>(rs + 128 + c * 32 + 4 * k);
