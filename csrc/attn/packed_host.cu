@@ -47,30 +47,47 @@ struct Bins {
   double makespan = 0.0;
 };
 
-// Longest item first to the least loaded block, one key/value head after the
-// other: blocks stay level and at any time work on the same few heads, whose
-// keys and values are then shared through L2.
-Bins balance(std::vector<Costed> one_head, int64_t kv_heads, int sms) {
-  std::stable_sort(one_head.begin(), one_head.end(), [](const Costed& a, const Costed& b) { return a.cost > b.cost; });
+// Items to the least loaded block, in the given order.
+Bins deal(const std::vector<Costed>& items, int sms) {
   Bins bins;
-  const int64_t total = static_cast<int64_t>(one_head.size()) * kv_heads;
-  const int n = static_cast<int>(std::min<int64_t>(sms, total));
-  bins.of.resize(std::max(n, 0));
+  const int n = static_cast<int>(std::min<size_t>(sms, items.size()));
+  bins.of.resize(n);
   using Load = std::pair<double, int>;
   std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
   for (int i = 0; i < n; ++i) least.emplace(0.0, i);
-  for (int64_t h = 0; h < kv_heads; ++h)
-    for (const Costed& c : one_head) {
-      Load l = least.top();
-      least.pop();
-      PackedItem item = c.item;
-      item.head = static_cast<int>(h);
-      bins.of[l.second].push_back(item);
-      l.first += c.cost;
-      bins.makespan = std::max(bins.makespan, l.first);
-      least.push(l);
-    }
+  for (const Costed& c : items) {
+    Load l = least.top();
+    least.pop();
+    bins.of[l.second].push_back(c.item);
+    l.first += c.cost;
+    bins.makespan = std::max(bins.makespan, l.first);
+    least.push(l);
+  }
   return bins;
+}
+
+// Longest first, one key/value head after the other: at any time the blocks work
+// on the same few heads, whose keys and values are then shared through L2.
+// With few heads that leaves blocks unlevel (8,324 + 4,109 causal tokens, 4 key
+// heads: the longest block 45 % over the mean); then longest first over all
+// heads, unless it gains less than 5 %.
+Bins balance(std::vector<Costed> one_head, int64_t kv_heads, int sms) {
+  auto longer = [](const Costed& a, const Costed& b) { return a.cost > b.cost; };
+  std::stable_sort(one_head.begin(), one_head.end(), longer);
+  std::vector<Costed> all;
+  all.reserve(one_head.size() * kv_heads);
+  for (int64_t h = 0; h < kv_heads; ++h)
+    for (Costed c : one_head) {
+      c.item.head = static_cast<int>(h);
+      all.push_back(c);
+    }
+  Bins by_head = deal(all, sms);
+  double total = 0.0;
+  for (const Costed& c : all) total += c.cost;
+  if (by_head.makespan * sms <= 1.05 * total) return by_head;
+  std::stable_sort(all.begin(), all.end(), longer);
+  Bins mixed = deal(all, sms);
+  return mixed.makespan * 1.05 < by_head.makespan ? mixed : by_head;
 }
 
 // Where whole items do not level the blocks (few rows over many keys): the
