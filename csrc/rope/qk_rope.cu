@@ -43,6 +43,7 @@ struct RopeParams {
   int runs, run;                // warps per token, heads (of q and k together) per warp
   long q_tok, q_head, k_tok, k_head;        // input strides (elements)
   long dq_tok, dq_head, dk_tok, dk_head;    // gradient input strides (backward)
+  long oq_tok, oq_head, ok_tok, ok_head;    // gradient output strides (backward)
   const float* positions;       // [T, axes] or null
   long pos_tok;
   const float* freqs;           // [end[kMaxAxes - 1]]
@@ -260,7 +261,8 @@ __global__ void __launch_bounds__(kThreads)
 // Heads [h0, h1) of one token: dy -> dx; adds to the lane's eight columns of the weight gradient.
 template <typename T, int D, bool INTER>
 __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long head, const T* __restrict__ dy,
-                                               long dy_head, T* __restrict__ dx, int h0, int h1, const void* w,
+                                               long dy_head, T* __restrict__ dx, long dx_head, int h0, int h1,
+                                               const void* w,
                                                const RopeParams& p, long t, bool& turned, float (&c)[4],
                                                float (&s)[4], float (&acc)[8]) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 2 : 1;
@@ -315,7 +317,7 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
         yb[i] = gb[i] * wb[i] - b[i] * (r * coef);
       }
       const int at = h + u * kGroups + g;
-      if (at < h1) store_pairs<D, INTER>(dx + at * D, l, ya, yb);
+      if (at < h1) store_pairs<D, INTER>(dx + at * dx_head, l, ya, yb);
     }
   }
 }
@@ -339,11 +341,11 @@ __global__ void __launch_bounds__(kThreads)
     float c[4], s[4];
     bool turned = false;
     if (h0 < p.Hq)
-      backward_heads<T, D, INTER>(q + t * p.q_tok, p.q_head, dyq + t * p.dq_tok, p.dq_head, dq + t * p.Hq * D, h0,
-                                  min(h1, p.Hq), qw, p, t, turned, c, s, acc[0]);
+      backward_heads<T, D, INTER>(q + t * p.q_tok, p.q_head, dyq + t * p.dq_tok, p.dq_head, dq + t * p.oq_tok,
+                                  p.oq_head, h0, min(h1, p.Hq), qw, p, t, turned, c, s, acc[0]);
     if (h1 > p.Hq)
-      backward_heads<T, D, INTER>(k + t * p.k_tok, p.k_head, dyk + t * p.dk_tok, p.dk_head, dk + t * p.Hk * D,
-                                  max(h0 - p.Hq, 0), h1 - p.Hq, kw, p, t, turned, c, s, acc[1]);
+      backward_heads<T, D, INTER>(k + t * p.k_tok, p.k_head, dyk + t * p.dk_tok, p.dk_head, dk + t * p.ok_tok,
+                                  p.ok_head, max(h0 - p.Hq, 0), h1 - p.Hq, kw, p, t, turned, c, s, acc[1]);
   }
   // Sum the lane groups in a fixed order: groups of a warp by shuffles, then the warps through shared memory.
   __shared__ float red[kThreads / 32][2 * D];
@@ -554,7 +556,7 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
                                          const at::Tensor& k_weight, const c10::optional<at::Tensor>& positions,
                                          const c10::optional<at::Tensor>& freqs, const std::vector<int64_t>& pairs,
                                          bool interleaved, const at::Tensor& dq_in, const at::Tensor& dk_in,
-                                         double eps) {
+                                         double eps, const std::vector<at::Tensor>& out) {
   const at::Tensor q = fit(q_in), k = fit(k_in), dq_out = fit(dq_in), dk_out = fit(dk_in);
   RopeParams p = make_params(q, k, positions, freqs, pairs, false, eps);
   bool kb = false;
@@ -566,8 +568,18 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
   TORCH_CHECK(dq_out.size(1) == q.size(1) && dk_out.size(1) == k.size(1), "dq and dk must have the heads of q and k");
   p.dq_tok = dq_out.stride(0), p.dq_head = dq_out.stride(1), p.dk_tok = dk_out.stride(0), p.dk_head = dk_out.stride(1);
   c10::cuda::CUDAGuard guard(q.get_device());
-  auto dq = empty_cuda(q.sizes(), q.scalar_type(), q);
-  auto dk = empty_cuda(k.sizes(), k.scalar_type(), k);
+  TORCH_CHECK(out.empty() || out.size() == 2, "out must hold dq and dk");
+  at::Tensor dq = out.empty() ? empty_cuda(q.sizes(), q.scalar_type(), q) : out[0];
+  at::Tensor dk = out.empty() ? empty_cuda(k.sizes(), k.scalar_type(), k) : out[1];
+  if (!out.empty()) {
+    check_heads(dq, "out dq", q);
+    check_heads(dk, "out dk", q);
+    TORCH_CHECK(dq.size(1) == q.size(1) && dk.size(1) == k.size(1), "out must have the heads of q and k");
+    for (const auto& t : out)
+      TORCH_CHECK((t.size(0) <= 1 || t.stride(0) > 0) && (t.size(1) <= 1 || t.stride(1) > 0),
+                  "out must not overlap itself");
+  }
+  p.oq_tok = dq.stride(0), p.oq_head = dq.stride(1), p.ok_tok = dk.stride(0), p.ok_head = dk.stride(1);
   const int heads = p.Hq + p.Hk, D = static_cast<int>(q.size(2));
   if (p.T == 0 || heads == 0) {
     auto zero = at::zeros({2, D}, q.options().dtype(at::kFloat));

@@ -15,11 +15,12 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q, const c10::optional<at:
                                     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& freqs,
                                     const std::vector<int64_t>& pairs, bool interleaved, bool inverse, double eps);
 
-// Gradients {dq, dk, dq_weight [D] fp32, dk_weight [D] fp32} of the normalising form.
+// Gradients {dq, dk, dq_weight [D] fp32, dk_weight [D] fp32} of the normalising
+// form; dq and dk go into `out` where it has two tensors.
 std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
                                          const at::Tensor& k_weight, const c10::optional<at::Tensor>& positions,
                                          const c10::optional<at::Tensor>& freqs, const std::vector<int64_t>& pairs,
                                          bool interleaved, const at::Tensor& dq_out, const at::Tensor& dk_out,
-                                         double eps);
+                                         double eps, const std::vector<at::Tensor>& out);
 
 }  // namespace h3

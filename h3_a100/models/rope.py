@@ -7,11 +7,18 @@ frame axis, so audio and video that play at the same moment share a phase;
 text tokens are unrotated.  Frequencies are ``base**(-2i/d_group)``.
 Tables are ``cos, sin: [T, head_dim/2]`` in fp32, in the token order
 ``[video | text | audio]`` used by the DiT.
+
+``axis_rope`` is the same rotation for a packed batch of samples of different
+sizes: the positions themselves, from which the kernels form the angles.
 """
 
 from __future__ import annotations
 
+from collections.abc import Iterable
+
 import torch
+
+from ..ops.packing import AxisRope
 
 
 def axis_pairs(head_dim: int) -> tuple[int, int, int]:
@@ -56,3 +63,24 @@ def rope_tables(
         audio = torch.zeros(0, pt + ph + pw, dtype=torch.float64)
     angles = torch.cat([video, text, audio], 0)
     return angles.cos().float().to(device), angles.sin().float().to(device)
+
+
+def axis_rope(
+    samples: Iterable[tuple[tuple[int, int, int], int, int]],
+    head_dim: int,
+    base: float = 10000.0,
+    device: torch.device | str = "cpu",
+) -> AxisRope:
+    """Rotation of packed samples, each ``(grid, n_text, n_audio)`` in the order ``[video | text | audio]``."""
+    parts = []
+    for (frames, height, width), n_text, n_audio in samples:
+        axes = [torch.arange(n, dtype=torch.float32) for n in (frames, height, width)]
+        parts.append(torch.stack(torch.meshgrid(*axes, indexing="ij"), -1).reshape(-1, 3))
+        parts.append(torch.zeros(n_text, 3))
+        times = torch.zeros(n_audio, 3)
+        times[:, 0] = torch.arange(n_audio, dtype=torch.float64) * (frames / max(n_audio, 1))
+        parts.append(times)
+    pairs = axis_pairs(head_dim)
+    positions = torch.cat(parts) if parts else torch.zeros(0, 3)
+    freqs = torch.cat([_freqs(n, base) for n in pairs]).float()
+    return AxisRope(positions.to(device), freqs.to(device), pairs)

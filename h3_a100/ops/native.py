@@ -216,10 +216,15 @@ class NativeKernels:
         both = self.C.qk_rope_fwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, False, float(eps))
         return both[0], both[1]
 
-    def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6):
-        """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32."""
+    def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6, out=None):
+        """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32.
+
+        ``out``: two tensors (views are fine) to write dq and dk into.  The
+        weights' sums run in a fixed order.
+        """
         pos, freqs, pairs, inter = self._rope_args(rope)
-        return tuple(self.C.qk_norm_rope_bwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, dq, dk, float(eps)))
+        return tuple(self.C.qk_norm_rope_bwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, dq, dk, float(eps),
+                                             [] if out is None else list(out)))
 
     def packed_plan(self, q_lens, k_lens=None, *, heads, kv_heads, head_dim, causal=False) -> PackedPlan:
         """Work lists of a packed batch, uploaded once; every layer's forward and backward uses them."""

@@ -263,8 +263,11 @@ class TorchKernels:
             out.append(self._turn(n, cos, sin, rope is None or rope.interleaved).to(x.dtype))
         return tuple(out)
 
-    def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6):
-        """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32."""
+    def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6, out=None):
+        """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32.
+
+        ``out``: two tensors (views are fine) to write dq and dk into.
+        """
         cos, sin = self._axis_tables(rope, q.shape[-1], q)
         grads, weights = [], []
         for x, w, dy in ((q, q_weight, dq), (k, k_weight, dk)):
@@ -275,6 +278,8 @@ class TorchKernels:
             gw = g * w.to(cos.dtype)
             grads.append((r * (gw - n * (gw * n).mean(-1, keepdim=True))).to(x.dtype))
             weights.append((g * n).sum((0, 1)))
+        if out is not None:
+            grads = [o.copy_(g) for o, g in zip(out, grads)]
         return grads[0], grads[1], weights[0], weights[1]
 
     def packed_plan(self, q_lens, k_lens=None, *, heads, kv_heads, head_dim, causal=False) -> PackedPlan:

@@ -509,3 +509,43 @@ def test_attention_refusals(K):
             K.attention_packed_bwd(q, k, v, *args, plan)
     with pytest.raises(RuntimeError, match="dq, dk and dv"):
         K.attention_packed_bwd(q, k, v, o, lse, q, plan, out=(q,))
+
+
+@gpu
+def test_out_views_and_their_refusals(K):
+    torch.manual_seed(14)
+    rope = rope_of(50, 64, 3, True, "cuda")
+    q, k, dq, dk, w = bf(50, 4, 64), bf(50, 2, 64), bf(50, 4, 64), bf(50, 2, 64), bf(64)
+    want = K.qk_norm_rope_bwd(q, k, w, w, rope, dq, dk)
+    fused = torch.full((50, 7 * 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = fused[:, :256].view(50, 4, 64), fused[:, 256:384].view(50, 2, 64)
+    got = K.qk_norm_rope_bwd(q, k, w, w, rope, dq, dk, out=out)
+    assert got[0].data_ptr() == out[0].data_ptr() and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert (fused[:, 384:] == 7.0).all()
+    for bad, message in (((out[0],), "dq and dk"), ((out[0], out[0]), "heads of q and k"), ((out[0].float(), out[1]), "type"),
+                         ((fused[:, 1:257].view(50, 4, 64), out[1]), "16-byte")):
+        with pytest.raises(RuntimeError, match=message):
+            K.qk_norm_rope_bwd(q, k, w, w, rope, dq, dk, out=bad)
+
+
+@gpu
+def test_checked_build_agrees(K):
+    """The bounds-checked build gives the same bits and reports nothing."""
+    try:
+        from h3_a100 import _C_checked
+    except ImportError:
+        pytest.skip("bounds-checked extension not built (H3_CHECKED_BUILD=1 python setup.py build_ext --inplace)")
+    from h3_a100.ops.native import NativeKernels
+
+    checked = NativeKernels(torch.device("cuda", 0), wait_limit_s=2.0, extension=_C_checked)
+    torch.manual_seed(15)
+    for q_lens, k_lens, heads, kv, dim, causal in (([77, 1, 300], None, 6, 2, 128, True), ([1, 2], [9000, 400], 8, 2, 64, True)):
+        plan = K.packed_plan(q_lens, k_lens, heads=heads, kv_heads=kv, head_dim=dim, causal=causal)
+        q, k, v = make(plan)
+        do = bf(plan.q_tokens, heads, dim)
+        results = []
+        for kernels in (K, checked):
+            o, lse = kernels.attention_packed_fwd(q, k, v, plan)
+            results.append((o, lse) + kernels.attention_packed_bwd(q, k, v, o, lse, do, plan))
+            kernels.check_status()
+        assert all(torch.equal(a, b) for a, b in zip(*results))
