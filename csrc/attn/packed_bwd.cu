@@ -26,6 +26,7 @@
 // TMEM columns: dq   dQ [0,128)  S [128,256)  dP, dS two buffers [256,512)
 //               dkv  dV [0,128)  dK [128,256)  S^T [256,384)  dP^T, then P^T and dS^T [384,512)
 // Every wait is bounded (ptx.cuh); every TMA load targets one CTA only.
+#include "../common/launch.h"
 #include "../common/ptx.cuh"
 #include "packed.h"
 #include "tile.cuh"
@@ -113,32 +114,41 @@ __device__ __forceinline__ void give_up(const KernelStatus& st, volatile int* ab
 // that 2^(s - lse2) = 0), both [Hk, Tq, G].  D / 8 lanes per row.
 template <int D>
 __global__ void __launch_bounds__(256) packed_delta_kernel(PackedBwdParams p) {
-  constexpr int kLanes = D / 8;
-  const long item = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  constexpr int kLanes = D / 8, kRows = 4, kGroups = 256 / kLanes;     // four rows a lane: eight loads in flight
   const int l = threadIdx.x % kLanes;
-  const bool live = item < p.Tq * p.Hq;
-  const long t = live ? item / p.Hq : 0;
-  const int h = live ? static_cast<int>(item - t * p.Hq) : 0;
-  float s = 0.f;
-  if (live) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p.o + t * p.o_tok + h * p.o_head + l * 8));
-    const uint4 b = *reinterpret_cast<const uint4*>(p.dout + t * p.do_tok + h * p.do_head + l * 8);
-    const __nv_bfloat162* a2 = reinterpret_cast<const __nv_bfloat162*>(&a);
-    const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&b);
+  const long base = static_cast<long>(blockIdx.x) * (kGroups * kRows) + threadIdx.x / kLanes;
+  uint4 a[kRows], b[kRows];
+  wait_for_prior();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 x = __bfloat1622float2(a2[i]), y = __bfloat1622float2(b2[i]);
-      s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-    }
+  for (int i = 0; i < kRows; ++i) {
+    const long item = base + i * kGroups;
+    const bool live = item < p.Tq * p.Hq;
+    const long t = live ? item / p.Hq : 0;
+    const int h = live ? static_cast<int>(item - t * p.Hq) : 0;
+    a[i] = __ldcs(reinterpret_cast<const uint4*>(p.o + t * p.o_tok + h * p.o_head + l * 8));
+    b[i] = *reinterpret_cast<const uint4*>(p.dout + t * p.do_tok + h * p.do_head + l * 8);
   }
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (live && l == 0) {
-    const int kh = h / p.G, g = h - kh * p.G;
-    const long at = (kh * p.Tq + t) * p.G + g;
-    const float lse = p.lse[h * p.Tq + t];
-    p.delta[at] = s;
-    p.lse2[at] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+  for (int i = 0; i < kRows; ++i) {
+    const __nv_bfloat162* a2 = reinterpret_cast<const __nv_bfloat162*>(&a[i]);
+    const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&b[i]);
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = __bfloat1622float2(a2[k]), y = __bfloat1622float2(b2[k]);
+      s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const long item = base + i * kGroups;
+    if (item < p.Tq * p.Hq && l == 0) {
+      const long t = item / p.Hq;
+      const int h = static_cast<int>(item - t * p.Hq), kh = h / p.G, g = h - kh * p.G;
+      const long at = (kh * p.Tq + t) * p.G + g;
+      const float lse = p.lse[h * p.Tq + t];
+      p.delta[at] = s;
+      p.lse2[at] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+    }
   }
 }
 
@@ -202,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_prior();
   const int begin = own.begin, end = own.end;
   if (warp < 4) {
     setmaxnreg_dec<kRegsLow>();
@@ -503,6 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_prior();
   const int begin = own.begin, end = own.end;
   // Query tiles of an item and live rows of the last one.
   auto query_tiles = [&](const PackedItem& it, int& last_rows) {
@@ -805,22 +817,22 @@ const char* packed_bwd_configure() {
 }
 
 void launch_packed_delta(int head_dim, const PackedBwdParams& p, cudaStream_t stream) {
-  const long threads = p.Tq * p.Hq * (head_dim / 8);
-  const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
-  if (head_dim == 128) packed_delta_kernel<128><<<blocks, 256, 0, stream>>>(p);
-  else packed_delta_kernel<64><<<blocks, 256, 0, stream>>>(p);
+  const long rows = 4L * 256 / (head_dim / 8);     // per block
+  const unsigned blocks = static_cast<unsigned>((p.Tq * p.Hq + rows - 1) / rows);
+  if (head_dim == 128) launch_overlapped(packed_delta_kernel<128>, blocks, 256, 0, stream, p);
+  else launch_overlapped(packed_delta_kernel<64>, blocks, 256, 0, stream, p);
 }
 
 void launch_packed_dq(int head_dim, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                       const CUtensorMap& dout, const PackedBwdParams& p, cudaStream_t stream) {
-  if (head_dim == 128) packed_dq_kernel<128><<<blocks, kThreads, Bwd<128>::kSmem, stream>>>(q, k, v, dout, p);
-  else packed_dq_kernel<64><<<blocks, kThreads, Bwd<64>::kSmem, stream>>>(q, k, v, dout, p);
+  if (head_dim == 128) launch_overlapped(packed_dq_kernel<128>, blocks, kThreads, Bwd<128>::kSmem, stream, q, k, v, dout, p);
+  else launch_overlapped(packed_dq_kernel<64>, blocks, kThreads, Bwd<64>::kSmem, stream, q, k, v, dout, p);
 }
 
 void launch_packed_dkv(int head_dim, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                        const CUtensorMap& dout, const PackedBwdParams& p, cudaStream_t stream) {
-  if (head_dim == 128) packed_dkv_kernel<128><<<blocks, kThreads, Bwd<128>::kSmem, stream>>>(q, k, v, dout, p);
-  else packed_dkv_kernel<64><<<blocks, kThreads, Bwd<64>::kSmem, stream>>>(q, k, v, dout, p);
+  if (head_dim == 128) launch_overlapped(packed_dkv_kernel<128>, blocks, kThreads, Bwd<128>::kSmem, stream, q, k, v, dout, p);
+  else launch_overlapped(packed_dkv_kernel<64>, blocks, kThreads, Bwd<64>::kSmem, stream, q, k, v, dout, p);
 }
 
 }  // namespace h3

@@ -29,6 +29,7 @@
 // issued at once and is ready before that warpgroup has finished its current
 // exponentials.  With P over the consumed S columns (S_0 S_1 in 256 columns) the
 // next S_t had to wait for PV_t, and a step was the chain softmax -> PV -> S.
+#include "../common/launch.h"
 #include "../common/ptx.cuh"
 #include "packed.h"
 #include "tile.cuh"
@@ -489,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_prior();
   if (warp < 4) {
     setmaxnreg_dec<kRegsLow>();
     if (warp == 0) {
@@ -522,6 +524,7 @@ template <int D>
 __global__ void __launch_bounds__(128) packed_join_kernel(const PackedJoin* __restrict__ list, PackedFwdParams p) {
   constexpr int kPer = D / 32;
   const PackedJoin jn = list[blockIdx.x];
+  wait_for_prior();
   const int rows = jn.nq * p.G, lane = lane_id();
   for (int row = blockIdx.y * 4 + warp_id(); row < rows; row += gridDim.y * 4) {
     const long first = static_cast<long>(jn.slot0) * p.part_rows + row;
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const PackedJoin* __re
 template <int D>
 void fwd(int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const PackedFwdParams& p,
          cudaStream_t stream) {
-  packed_fwd_kernel<D><<<blocks, kThreads, Fwd<D>::kSmem, stream>>>(q, k, v, p);
+  launch_overlapped(packed_fwd_kernel<D>, blocks, kThreads, Fwd<D>::kSmem, stream, q, k, v, p);
 }
 
 template <int D>
@@ -611,8 +614,8 @@ void launch_packed_fwd(int head_dim, int blocks, const CUtensorMap& q, const CUt
 void launch_packed_join(int head_dim, int joins, const PackedJoin* list, const PackedFwdParams& p,
                         cudaStream_t stream) {
   const dim3 grid(joins, (p.part_rows + 3) / 4);
-  if (head_dim == 128) packed_join_kernel<128><<<grid, 128, 0, stream>>>(list, p);
-  else packed_join_kernel<64><<<grid, 128, 0, stream>>>(list, p);
+  if (head_dim == 128) launch_overlapped(packed_join_kernel<128>, grid, 128, 0, stream, list, p);
+  else launch_overlapped(packed_join_kernel<64>, grid, 128, 0, stream, list, p);
 }
 
 }  // namespace h3

@@ -246,6 +246,7 @@ __global__ void __launch_bounds__(kThreads)
                        const void* __restrict__ kw, T* __restrict__ q_out, T* __restrict__ k_out, RopeParams p) {
   const long warp = static_cast<long>(blockIdx.x) * (kThreads / 32) + warp_id();
   const long t = warp / p.runs;
+  wait_for_prior();
   if (t >= p.T) return;
   const int h0 = static_cast<int>(warp - t * p.runs) * p.run, h1 = min(h0 + p.run, p.Hq + p.Hk);
   float c[4], s[4];
@@ -334,6 +335,7 @@ __global__ void __launch_bounds__(kThreads)
   float acc[2][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.f;
+  wait_for_prior();
   const long warps = static_cast<long>(gridDim.x) * (kThreads / 32), total = p.T * p.runs;
   for (long i = static_cast<long>(blockIdx.x) * (kThreads / 32) + warp_id(); i < total; i += warps) {
     const long t = i / p.runs;
@@ -375,6 +377,7 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* __restr
   __shared__ float s[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
+  wait_for_prior();
 #pragma unroll 8
   for (int r = threadIdx.y; r < rows; r += 32) v += partial[static_cast<long>(r) * 2 * D + c];
   s[threadIdx.y][threadIdx.x] = v;
@@ -540,9 +543,9 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q_in, const c10::optional<
     constexpr int kD = decltype(dim)::value;
     constexpr bool kInter = decltype(inter)::value;
     auto args = [&](auto kernel) {
-      kernel<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-          reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
-          reinterpret_cast<T*>(q_out.data_ptr()), reinterpret_cast<T*>(k_out.data_ptr()), p);
+      launch_overlapped(kernel, static_cast<unsigned>(blocks), kThreads, 0, stream,
+                        reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
+                        reinterpret_cast<T*>(q_out.data_ptr()), reinterpret_cast<T*>(k_out.data_ptr()), p);
     };
     if (qw != nullptr) args(qk_rope_fwd_kernel<T, kD, kInter, true>);
     else args(qk_rope_fwd_kernel<T, kD, kInter, false>);
@@ -596,14 +599,14 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
     const long blocks = (p.T * p.runs + kThreads / 32 - 1) / (kThreads / 32);
     const int grid = static_cast<int>(std::min<long>(blocks, resident_blocks(kernel)));
     auto partial = empty_cuda({grid, 2 * kD}, at::kFloat, q);
-    kernel<<<grid, kThreads, 0, stream>>>(
-        reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
+    launch_overlapped(
+        kernel, grid, kThreads, 0, stream, reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
         reinterpret_cast<const T*>(dq_out.data_ptr()), reinterpret_cast<const T*>(dk_out.data_ptr()),
         reinterpret_cast<T*>(dq.data_ptr()), reinterpret_cast<T*>(dk.data_ptr()), partial.data_ptr<float>(), p);
     note_launch();
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    sum_partials_kernel<<<2 * kD / 32, dim3(32, 32), 0, stream>>>(partial.data_ptr<float>(), grid, kD,
-                                                                  dqw.data_ptr<float>(), dkw.data_ptr<float>());
+    launch_overlapped(sum_partials_kernel, 2 * kD / 32, dim3(32, 32), 0, stream, partial.data_ptr<float>(), grid, kD,
+                      dqw.data_ptr<float>(), dkw.data_ptr<float>());
     note_launch();
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
