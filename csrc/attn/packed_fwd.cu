@@ -64,6 +64,8 @@ struct Bars {
   uint64_t *s_taken;     // S is in its warpgroup's registers, the columns are free
   uint64_t *p_full;      // [t] P_t is in TMEM
   uint64_t *pv_done;     // [t] PV_t is complete
+  uint64_t *traded;      // [t] warpgroup t has put its m and l up for the other
+  uint64_t *joined;      // [t] warpgroup t has read both accumulators
   uint64_t *drain;       // [2] the issuers' last products are complete
 };
 
@@ -296,12 +298,14 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
   const uint32_t lane_off = static_cast<uint32_t>((warp_id() & 3) * 32) << 16;
   const uint32_t tS = tmem + lane_off, tP = tmem + 128 + t * 64 + lane_off, tO = tmem + 256 + lane_off;
   const int tok = row / p.G, g = row - tok * p.G;   // token of the tile and head of the group of this row
-  int steps = 0;          // this warpgroup's key tiles so far
+  int steps = 0, other_steps = 0;     // key tiles so far of this warpgroup and of the other
+  int trades = 0;                     // items that both worked on
   bool ok = true;
   for (int i = own.begin; i < own.end; ++i) {
     const PackedItem it = own.item(p, i);
     const TileWork w = tile_work(it, p.bt);
     const int first = w.solo ? 0 : t * p.bt, n_kv = w.n(t);
+    other_steps += w.n(t ^ 1);
     const bool both = w.solo && w.n1 > 0;      // one query tile, both warpgroups on it
     if (w.solo ? t == 1 && !both : it.nq <= first) continue;
     const bool live = row < min(p.bt, it.nq - first) * p.G;
@@ -359,16 +363,14 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
       tc_fence_before();
       warp_arrive(&b.p_full[t]);
     }
-    if (ok && n_kv > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&b.pv_done[t], (steps - 1) & 1, limit, abort_flag));
-    }
     if (!ok) break;
-    tc_fence_after();
     float scale_own = 1.f, scale_other = 0.f;
     if (both) {
       // Join the two accumulators of the row; each warpgroup then writes half of the columns.
       exchange[t * 128 + row] = make_float2(m, l);
-      named_bar_sync(2, 256);
+      warp_arrive(&b.traded[t]);
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.traded[t ^ 1], trades & 1, limit, abort_flag));
+      if (!ok) break;
       const float2 other = exchange[(t ^ 1) * 128 + row];
       const float top = fmaxf(m, other.x);
       scale_own = m == -INFINITY ? 0.f : ex2(m - top);
@@ -386,15 +388,29 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
     const bool part = it.slot >= 0;
     const long part_row = (static_cast<long>(it.slot) + (w.solo ? 0 : t * it.pad)) * p.part_rows + row;
     const long o_off = part ? part_row * D : (q * p.Hq + head) * D;
-    // 32 TMEM columns a wait (the register budget): 32 of this row's O_t, or 16 of each accumulator.
-    const int first_col = both ? t * (D / 2) : 0, cols = both ? D / 2 : D, step = both ? 16 : 32;
-#pragma unroll 1
-    for (int c = 0; c < cols; c += step) {
-      const int col = first_col + c;
-      uint32_t r[2][16];      // without a key tile (`some` is false then): whatever is there
-      tmem_ld16(tO + t * 128 + col, r[0]);
-      tmem_ld16(both ? tO + (t ^ 1) * 128 + col : tO + t * 128 + col + 16, r[1]);
-      tmem_ld_wait();
+    const long lse_off = static_cast<long>(head) * p.Tq + q;
+    if (!both || t == 0) {
+      if (live && part) {
+        p.part_lse[part_row] = lse2;
+      } else if (live && H3_IN_BOUNDS(lse_off, lse_off, p.lse_extent, p.status)) {
+        p.lse[lse_off] = lse2 * 0.6931471805599453f;
+      }
+    }
+    // The accumulators are complete (all of the above ran beside the last product).
+    ok = __all_sync(0xffffffffu,
+                    (n_kv == 0 || mbar_wait(&b.pv_done[t], (steps - 1) & 1, limit, abort_flag)) &&
+                        (!both || mbar_wait(&b.pv_done[t ^ 1], (other_steps - 1) & 1, limit, abort_flag)));
+    if (!ok) break;
+    tc_fence_after();
+    // 32 TMEM columns at a time: 32 of this row's O_t, or 16 of each accumulator; the next ones are on their way
+    // while these are written.  Without a key tile (`some` is false then) they hold whatever is there.
+    const int first_col = both ? t * (D / 2) : 0, step = both ? 16 : 32;
+    const uint32_t left = tO + t * 128 + first_col, right = both ? tO + (t ^ 1) * 128 + first_col : left + 16;
+    auto fetch = [&](int c, uint32_t (&r)[2][16]) {
+      tmem_ld16(left + c * step, r[0]);
+      tmem_ld16(right + c * step, r[1]);
+    };
+    auto emit = [&](int c, uint32_t (&r)[2][16]) {
       if (both) {
 #pragma unroll
         for (int k = 0; k < 16; ++k)
@@ -406,7 +422,7 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
         float v[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = some ? __uint_as_float(r[h][k]) * (both ? 1.f : scale_own) : 0.f;
-        const long at = o_off + col + h * 16;
+        const long at = o_off + first_col + c * step + h * 16;
         if (!live || !H3_IN_BOUNDS(at, at + 15, part ? p.part_extent : p.o_extent, p.status)) continue;
         if (part) {
 #pragma unroll
@@ -420,17 +436,26 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
           store16_bf16(p.o + at, v, true);      // o is contiguous, allocated here
         }
       }
-    }
-    const long lse_off = static_cast<long>(head) * p.Tq + q;
-    if (!both || t == 0) {
-      if (live && part) {
-        p.part_lse[part_row] = lse2;
-      } else if (live && H3_IN_BOUNDS(lse_off, lse_off, p.lse_extent, p.status)) {
-        p.lse[lse_off] = lse2 * 0.6931471805599453f;
-      }
+    };
+    uint32_t ra[2][16], rb[2][16];
+    fetch(0, ra);
+    tmem_ld_wait();
+#pragma unroll 1
+    for (int c = 0; c < D / 32; c += 2) {
+      fetch(c + 1, rb);
+      emit(c, ra);
+      tmem_ld_wait();
+      if (c + 2 < D / 32) fetch(c + 2, ra);
+      emit(c + 1, rb);
+      tmem_ld_wait();
     }
     tc_fence_before();
-    if (both) named_bar_sync(2, 256);    // both accumulators and the exchange are free again
+    if (both) {     // both accumulators and the exchange are free again
+      warp_arrive(&b.joined[t]);
+      ok = __all_sync(0xffffffffu, mbar_wait(&b.joined[t ^ 1], trades & 1, limit, abort_flag));
+      ++trades;
+      if (!ok) break;
+    }
   }
   if (!ok) {
     if (lane_id() == 0) report_status(p.status, kStatusTimeoutAccFull, steps);
@@ -457,9 +482,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   b.pv_done = bars + 8;
   b.drain = bars + 10;
   b.s_taken = bars + 12;
-  rk.place(bars + 13, sQ + 2 * C::kTile);
-  rv.place(bars + 13 + rk.kBarriers, rk.base + C::kK * C::kTile);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13 + rk.kBarriers + rv.kBarriers);
+  b.traded = bars + 13;
+  b.joined = bars + 15;
+  rk.place(bars + 17, sQ + 2 * C::kTile);
+  rv.place(bars + 17 + rk.kBarriers, rk.base + C::kK * C::kTile);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17 + rk.kBarriers + rv.kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id();
   const Slice own(p.items, p.begin);
@@ -469,6 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b.q_empty[t], 1);
       mbar_init(&b.s_full[t], 1);
       mbar_init(&b.p_full[t], 4);
+      mbar_init(&b.traded[t], 4);
+      mbar_init(&b.joined[t], 4);
       mbar_init(&b.pv_done[t], 1);
     }
     rk.init();
