@@ -117,15 +117,16 @@ template <int D>
 __global__ void __launch_bounds__(256) packed_delta_kernel(PackedBwdParams p) {
   constexpr int kLanes = D / 8, kRows = 4, kGroups = 256 / kLanes;     // four rows a lane: eight loads in flight
   const int l = threadIdx.x % kLanes;
-  const long base = static_cast<long>(blockIdx.x) * (kGroups * kRows) + threadIdx.x / kLanes;
+  // The block's first row by one 64-bit division, the others from it in 32 bits.
+  const long first = static_cast<long>(blockIdx.x) * (kGroups * kRows);
+  const long t0 = first / p.Hq;
+  const int h0 = static_cast<int>(first - t0 * p.Hq);
   uint4 a[kRows], b[kRows];
   wait_for_prior();
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const long item = base + i * kGroups;
-    const bool live = item < p.Tq * p.Hq;
-    const long t = live ? item / p.Hq : 0;
-    const int h = live ? static_cast<int>(item - t * p.Hq) : 0;
+    const int at = h0 + threadIdx.x / kLanes + i * kGroups, up = at / p.Hq, h = at - up * p.Hq;
+    const long t = min(t0 + up, p.Tq - 1);      // rows past the last one are read and not written
     a[i] = __ldcs(reinterpret_cast<const uint4*>(p.o + t * p.o_tok + h * p.o_head + l * 8));
     b[i] = *reinterpret_cast<const uint4*>(p.dout + t * p.do_tok + h * p.do_head + l * 8);
   }
@@ -141,14 +142,14 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(PackedBwdParams p) {
     }
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const long item = base + i * kGroups;
-    if (item < p.Tq * p.Hq && l == 0) {
-      const long t = item / p.Hq;
-      const int h = static_cast<int>(item - t * p.Hq), kh = h / p.G, g = h - kh * p.G;
-      const long at = (kh * p.Tq + t) * p.G + g;
+    const int at = h0 + threadIdx.x / kLanes + i * kGroups, up = at / p.Hq, h = at - up * p.Hq;
+    const long t = t0 + up;
+    if (t < p.Tq && l == 0) {
+      const int kh = h / p.G, g = h - kh * p.G;
+      const long row = (kh * p.Tq + t) * p.G + g;
       const float lse = p.lse[h * p.Tq + t];
-      p.delta[at] = s;
-      p.lse2[at] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+      p.delta[row] = s;
+      p.lse2[row] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
     }
   }
 }

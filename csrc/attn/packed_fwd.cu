@@ -547,6 +547,42 @@ __global__ void __launch_bounds__(kThreads, 1)
   named_bar_sync(1, kThreads);
 }
 
+// Adds parts [0, parts) of a row, BATCH parts' loads at a time: a row waits for memory once per batch.
+template <int PER, int BATCH>
+__device__ __forceinline__ void add_parts(const float* __restrict__ o, const float* __restrict__ lses, long stride,
+                                          int parts, float& m, float& sum, float (&acc)[PER]) {
+  for (int i0 = 0; i0 < parts; i0 += BATCH) {
+    float lse[BATCH], v[BATCH][PER], top = m;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const bool have = i0 + i < parts;
+      lse[i] = have ? lses[(i0 + i) * stride] : -INFINITY;
+      const float* src = o + (i0 + i) * stride * (32 * PER);
+      if (PER == 4) {
+        const float4 u = have ? *reinterpret_cast<const float4*>(src) : float4{};
+        v[i][0] = u.x, v[i][1] = u.y, v[i][PER - 2] = u.z, v[i][PER - 1] = u.w;
+      } else {
+        const float2 u = have ? *reinterpret_cast<const float2*>(src) : float2{};
+        v[i][0] = u.x, v[i][1] = u.y;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) top = fmaxf(top, lse[i]);
+    const float base = top == -INFINITY ? 0.f : top, old = ex2(m - base);
+    m = top;
+    sum *= old;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) acc[k] *= old;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float weight = ex2(lse[i] - base);
+      sum += weight;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] = fmaf(weight, v[i][k], acc[k]);
+    }
+  }
+}
+
 // o = sum_i 2^(lse_i - lse) o_i over the parts of a split row, in the order of
 // the parts; one warp per row.
 template <int D>
@@ -557,40 +593,12 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const PackedJoin* __re
   const int rows = jn.nq * p.G, lane = lane_id();
   for (int row = blockIdx.y * 4 + warp_id(); row < rows; row += gridDim.y * 4) {
     const long first = static_cast<long>(jn.slot0) * p.part_rows + row;
+    const float *o = p.part_o + first * D + lane * kPer, *lses = p.part_lse + first;
     float m = -INFINITY, sum = 0.f, acc[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-    // Four parts' loads at a time: most rows have no more, and wait for memory once.
-    for (int i0 = 0; i0 < jn.parts; i0 += 4) {
-      float lse[4], v[4][kPer], top = m;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool have = i0 + i < jn.parts;
-        const long r = first + static_cast<long>(i0 + i) * p.part_rows;
-        lse[i] = have ? p.part_lse[r] : -INFINITY;
-        if (kPer == 4) {
-          const float4 u = have ? *reinterpret_cast<const float4*>(p.part_o + r * D + lane * kPer) : float4{};
-          v[i][0] = u.x, v[i][1] = u.y, v[i][kPer - 2] = u.z, v[i][kPer - 1] = u.w;
-        } else {
-          const float2 u = have ? *reinterpret_cast<const float2*>(p.part_o + r * D + lane * kPer) : float2{};
-          v[i][0] = u.x, v[i][1] = u.y;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, lse[i]);
-      const float base = top == -INFINITY ? 0.f : top, old = ex2(m - base);
-      m = top;
-      sum *= old;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[k] *= old;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float weight = ex2(lse[i] - base);
-        sum += weight;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(weight, v[i][k], acc[k]);
-      }
-    }
+    if (jn.parts <= 2) add_parts<kPer, 2>(o, lses, p.part_rows, jn.parts, m, sum, acc);   // prompts: cut once
+    else add_parts<kPer, 4>(o, lses, p.part_rows, jn.parts, m, sum, acc);
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     const int tok = row / p.G, head = jn.head * p.G + row - tok * p.G;
     const long q = static_cast<long>(jn.q0) + tok;
