@@ -85,48 +85,87 @@ __device__ __forceinline__ Raw<float> load_pairs(const float* p, int l) {
   return r;
 }
 
-__device__ __forceinline__ float2 unpack(uint32_t u) {
-  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
+// The four pairs are computed two at a time in packed f32x2 instructions: half
+// the issues, which under the power cap is clock (sustained passes: 37,730
+// tokens 269.5 -> 267.0 us, training 156.4 -> 155.0 us).
+struct Four {
+  uint64_t v[2];
+};
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ Four fma4(const Four& a, const Four& b, const Four& c) {
+  Four d;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v[i]) : "l"(a.v[i]), "l"(b.v[i]), "l"(c.v[i]));
+  return d;
+}
+__device__ __forceinline__ Four mul4(const Four& a, const Four& b) {
+  Four d;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v[i]) : "l"(a.v[i]), "l"(b.v[i]));
+  return d;
+}
+__device__ __forceinline__ Four four(float x, float y, float z, float w) { return {{pack2(x, y), pack2(z, w)}}; }
+__device__ __forceinline__ Four all4(float x) { return four(x, x, x, x); }
+__device__ __forceinline__ float sum4(const Four& a) {
+  const float2 x = unpack2(a.v[0]), y = unpack2(a.v[1]);
+  return (x.x + x.y) + (y.x + y.y);
 }
 
+__device__ __forceinline__ float low(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+// First and second members of a lane's pairs.
 template <bool INTER>
-__device__ __forceinline__ void split(const Raw<__nv_bfloat16>& r, float (&a)[4], float (&b)[4]) {
-  const float2 e0 = unpack(r.lo.x), e1 = unpack(r.lo.y), e2 = unpack(r.hi.x), e3 = unpack(r.hi.y);
+__device__ __forceinline__ void split(const Raw<__nv_bfloat16>& r, Four& a, Four& b) {
   if (INTER) {
-    a[0] = e0.x, b[0] = e0.y, a[1] = e1.x, b[1] = e1.y, a[2] = e2.x, b[2] = e2.y, a[3] = e3.x, b[3] = e3.y;
+    a = four(low(r.lo.x), low(r.lo.y), low(r.hi.x), low(r.hi.y));
+    b = four(high(r.lo.x), high(r.lo.y), high(r.hi.x), high(r.hi.y));
   } else {
-    a[0] = e0.x, a[1] = e0.y, a[2] = e1.x, a[3] = e1.y, b[0] = e2.x, b[1] = e2.y, b[2] = e3.x, b[3] = e3.y;
+    a = four(low(r.lo.x), high(r.lo.x), low(r.lo.y), high(r.lo.y));
+    b = four(low(r.hi.x), high(r.hi.x), low(r.hi.y), high(r.hi.y));
   }
 }
 template <bool INTER>
-__device__ __forceinline__ void split(const Raw<float>& r, float (&a)[4], float (&b)[4]) {
+__device__ __forceinline__ void split(const Raw<float>& r, Four& a, Four& b) {
   if (INTER) {
-    a[0] = r.lo.x, b[0] = r.lo.y, a[1] = r.lo.z, b[1] = r.lo.w;
-    a[2] = r.hi.x, b[2] = r.hi.y, a[3] = r.hi.z, b[3] = r.hi.w;
+    a = four(r.lo.x, r.lo.z, r.hi.x, r.hi.z);
+    b = four(r.lo.y, r.lo.w, r.hi.y, r.hi.w);
   } else {
-    a[0] = r.lo.x, a[1] = r.lo.y, a[2] = r.lo.z, a[3] = r.lo.w;
-    b[0] = r.hi.x, b[1] = r.hi.y, b[2] = r.hi.z, b[3] = r.hi.w;
+    a = four(r.lo.x, r.lo.y, r.lo.z, r.lo.w);
+    b = four(r.hi.x, r.hi.y, r.hi.z, r.hi.w);
   }
 }
 
 template <int D, bool INTER>
-__device__ __forceinline__ void store_pairs(__nv_bfloat16* p, int l, const float (&a)[4], const float (&b)[4]) {
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* p, int l, const Four& fa, const Four& fb) {
+  const float2 a0 = unpack2(fa.v[0]), a1 = unpack2(fa.v[1]), b0 = unpack2(fb.v[0]), b1 = unpack2(fb.v[1]);
   if (INTER) {
-    *reinterpret_cast<uint4*>(p + 8 * l) = make_uint4(pack_bf16x2(a[0], b[0]), pack_bf16x2(a[1], b[1]),
-                                                      pack_bf16x2(a[2], b[2]), pack_bf16x2(a[3], b[3]));
+    *reinterpret_cast<uint4*>(p + 8 * l) =
+        make_uint4(pack_bf16x2(a0.x, b0.x), pack_bf16x2(a0.y, b0.y), pack_bf16x2(a1.x, b1.x), pack_bf16x2(a1.y, b1.y));
   } else {
-    *reinterpret_cast<uint2*>(p + 4 * l) = make_uint2(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]));
-    *reinterpret_cast<uint2*>(p + D / 2 + 4 * l) = make_uint2(pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3]));
+    *reinterpret_cast<uint2*>(p + 4 * l) = make_uint2(pack_bf16x2(a0.x, a0.y), pack_bf16x2(a1.x, a1.y));
+    *reinterpret_cast<uint2*>(p + D / 2 + 4 * l) = make_uint2(pack_bf16x2(b0.x, b0.y), pack_bf16x2(b1.x, b1.y));
   }
 }
 template <int D, bool INTER>
-__device__ __forceinline__ void store_pairs(float* p, int l, const float (&a)[4], const float (&b)[4]) {
+__device__ __forceinline__ void store_pairs(float* p, int l, const Four& fa, const Four& fb) {
+  const float2 a0 = unpack2(fa.v[0]), a1 = unpack2(fa.v[1]), b0 = unpack2(fb.v[0]), b1 = unpack2(fb.v[1]);
   if (INTER) {
-    *reinterpret_cast<float4*>(p + 8 * l) = make_float4(a[0], b[0], a[1], b[1]);
-    *reinterpret_cast<float4*>(p + 8 * l + 4) = make_float4(a[2], b[2], a[3], b[3]);
+    *reinterpret_cast<float4*>(p + 8 * l) = make_float4(a0.x, b0.x, a0.y, b0.y);
+    *reinterpret_cast<float4*>(p + 8 * l + 4) = make_float4(a1.x, b1.x, a1.y, b1.y);
   } else {
-    *reinterpret_cast<float4*>(p + 4 * l) = make_float4(a[0], a[1], a[2], a[3]);
-    *reinterpret_cast<float4*>(p + D / 2 + 4 * l) = make_float4(b[0], b[1], b[2], b[3]);
+    *reinterpret_cast<float4*>(p + 4 * l) = make_float4(a0.x, a0.y, a1.x, a1.y);
+    *reinterpret_cast<float4*>(p + D / 2 + 4 * l) = make_float4(b0.x, b0.y, b1.x, b1.y);
   }
 }
 
@@ -161,23 +200,27 @@ __device__ __forceinline__ void turn(const RopeParams& p, long t, int i, float& 
 // cos and sin of a lane's four pairs of token t.  The groups of a warp work on
 // the same token: each computes its share of the four and they exchange.
 template <int D>
-__device__ __forceinline__ void turns(const RopeParams& p, long t, int l, float (&c)[4], float (&s)[4]) {
+__device__ __forceinline__ void turns(const RopeParams& p, long t, int l, Four& cos4, Four& sin4) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kShare = 4 / kGroups;
   const int g = lane_id() / kLanes;
   float mc[kShare], ms[kShare];
 #pragma unroll
   for (int i = 0; i < kShare; ++i) turn(p, t, 4 * l + g * kShare + i, mc[i], ms[i]);
+  float c[4], s[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int from = (i / kShare) * kLanes + l;
     c[i] = __shfl_sync(0xffffffffu, mc[i % kShare], from);
     s[i] = __shfl_sync(0xffffffffu, ms[i % kShare], from);
   }
+  cos4 = four(c[0], c[1], c[2], c[3]);
+  sin4 = four(s[0], s[1], s[2], s[3]);
 }
 
 // A lane's weights, as the first and second members of its pairs.
 template <int D, bool INTER>
-__device__ __forceinline__ void weights(const void* w, bool bf16, int l, float (&a)[4], float (&b)[4]) {
+__device__ __forceinline__ void weights(const void* w, bool bf16, int l, Four& first4, Four& second4) {
+  float a[4], b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int first = INTER ? 2 * (4 * l + i) : 4 * l + i, second = INTER ? first + 1 : first + D / 2;
@@ -189,16 +232,18 @@ __device__ __forceinline__ void weights(const void* w, bool bf16, int l, float (
       b[i] = static_cast<const float*>(w)[second];
     }
   }
+  first4 = four(a[0], a[1], a[2], a[3]);
+  second4 = four(b[0], b[1], b[2], b[3]);
 }
 
 // Heads [h0, h1) of one token: x -> y (contiguous heads).
 template <typename T, int D, bool INTER, bool NORM>
 __device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head, T* __restrict__ y, int h0, int h1,
-                                              const void* w, const RopeParams& p, long t, bool& turned, float (&c)[4],
-                                              float (&s)[4]) {
+                                              const void* w, const RopeParams& p, long t, bool& turned, Four& c,
+                                              Four& s) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 4 : 2;
   const int g = lane_id() / kLanes, l = lane_id() % kLanes;
-  float wa[4], wb[4];
+  Four wa, wb;
   Raw<T> next[kBatch];
   auto fetch = [&](int h) {
 #pragma unroll
@@ -209,6 +254,7 @@ __device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head
   if (NORM) weights<D, INTER>(w, p.w_bf16, l, wa, wb);
   if (!turned) turns<D>(p, t, l, c, s);      // after the first loads are on their way
   turned = true;
+  const Four neg_s = mul4(s, all4(-1.f));
   for (int h = h0; h < h1; h += kBatch * kGroups) {
     Raw<T> now[kBatch];
 #pragma unroll
@@ -216,24 +262,15 @@ __device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head
     fetch(h + kBatch * kGroups);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      float a[4], b[4], ya[4], yb[4];
+      Four a, b;
       split<INTER>(now[u], a, b);
       if (NORM) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        const float r = rsqrtf(group_sum<kLanes>(ss) * (1.f / D) + p.eps);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] *= r * wa[i];
-          b[i] *= r * wb[i];
-        }
+        const float ss = group_sum<kLanes>(sum4(fma4(a, a, mul4(b, b))));
+        const Four r = all4(rsqrtf(ss * (1.f / D) + p.eps));
+        a = mul4(a, mul4(r, wa));
+        b = mul4(b, mul4(r, wb));
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ya[i] = a[i] * c[i] - b[i] * s[i];
-        yb[i] = a[i] * s[i] + b[i] * c[i];
-      }
+      const Four ya = fma4(b, neg_s, mul4(a, c)), yb = fma4(b, c, mul4(a, s));
       const int at = h + u * kGroups + g;
       if (at < h1) store_pairs<D, INTER>(y + at * D, l, ya, yb);
     }
@@ -249,7 +286,7 @@ __global__ void __launch_bounds__(kThreads)
   wait_for_prior();
   if (t >= p.T) return;
   const int h0 = static_cast<int>(warp - t * p.runs) * p.run, h1 = min(h0 + p.run, p.Hq + p.Hk);
-  float c[4], s[4];
+  Four c, s;
   bool turned = false;
   if (h0 < p.Hq)
     forward_heads<T, D, INTER, NORM>(q + t * p.q_tok, p.q_head, q_out + t * p.Hq * D, h0, min(h1, p.Hq), qw, p, t,
@@ -264,11 +301,11 @@ template <typename T, int D, bool INTER>
 __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long head, const T* __restrict__ dy,
                                                long dy_head, T* __restrict__ dx, long dx_head, int h0, int h1,
                                                const void* w,
-                                               const RopeParams& p, long t, bool& turned, float (&c)[4],
-                                               float (&s)[4], float (&acc)[8]) {
+                                               const RopeParams& p, long t, bool& turned, Four& c,
+                                               Four& s, Four (&acc)[2]) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 2 : 1;
   const int g = lane_id() / kLanes, l = lane_id() % kLanes;
-  float wa[4], wb[4];
+  Four wa, wb;
   Raw<T> next_x[kBatch], next_y[kBatch];
   auto fetch = [&](int h) {
 #pragma unroll
@@ -282,6 +319,7 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
   weights<D, INTER>(w, p.w_bf16, l, wa, wb);
   if (!turned) turns<D>(p, t, l, c, s);
   turned = true;
+  const Four neg_s = mul4(s, all4(-1.f));
   for (int h = h0; h < h1; h += kBatch * kGroups) {
     Raw<T> now_x[kBatch], now_y[kBatch];
 #pragma unroll
@@ -292,40 +330,30 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
     fetch(h + kBatch * kGroups);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      float a[4], b[4], ya[4], yb[4], ga[4], gb[4], ss = 0.f, gx = 0.f;
+      Four a, b, ya, yb;
       split<INTER>(now_x[u], a, b);
       split<INTER>(now_y[u], ya, yb);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ga[i] = ya[i] * c[i] + yb[i] * s[i];
-        gb[i] = yb[i] * c[i] - ya[i] * s[i];
-        ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        gx = fmaf(ga[i] * wa[i], a[i], fmaf(gb[i] * wb[i], b[i], gx));
-      }
+      const Four ga = fma4(yb, s, mul4(ya, c)), gb = fma4(ya, neg_s, mul4(yb, c));
+      const Four gwa = mul4(ga, wa), gwb = mul4(gb, wb);
       // Both sums before r is known, so that their shuffles overlap.
-      ss = group_sum<kLanes>(ss);
-      gx = group_sum<kLanes>(gx);
+      const float ss = group_sum<kLanes>(sum4(fma4(a, a, mul4(b, b))));
+      const float gx = group_sum<kLanes>(sum4(fma4(gwa, a, mul4(gwb, b))));
       // Rows past h1 are zeros: r is finite and everything below is zero.
       const float r = rsqrtf(ss * (1.f / D) + p.eps);
-      const float coef = r * r * (gx * (1.f / D));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ga[i] *= r;
-        gb[i] *= r;
-        acc[i] = fmaf(ga[i], a[i], acc[i]);
-        acc[4 + i] = fmaf(gb[i], b[i], acc[4 + i]);
-        ya[i] = ga[i] * wa[i] - a[i] * (r * coef);
-        yb[i] = gb[i] * wb[i] - b[i] * (r * coef);
-      }
+      const Four r4 = all4(r), back = all4(-r * r * r * (gx * (1.f / D)));
+      acc[0] = fma4(mul4(ga, r4), a, acc[0]);
+      acc[1] = fma4(mul4(gb, r4), b, acc[1]);
+      ya = fma4(a, back, mul4(gwa, r4));
+      yb = fma4(b, back, mul4(gwb, r4));
       const int at = h + u * kGroups + g;
       if (at < h1) store_pairs<D, INTER>(dx + at * dx_head, l, ya, yb);
     }
   }
 }
 
-// Five blocks of 128 threads an SM: 20 warps in about 100 registers a thread
-// (two blocks of 256 threads: 16 warps; 16,411 tokens 96.6 us against 93.4).
-constexpr int kBwdThreads = 128, kBwdBlocks = 5;
+// Four blocks of 128 threads an SM, 16 warps in up to 128 registers a thread; five blocks spill
+// (16,411 tokens, a sustained pass: 155.0 us against 162.0).
+constexpr int kBwdThreads = 128, kBwdBlocks = 4;
 
 // Backward.  Warps take (token, run of heads) in a grid stride, so that each
 // block leaves one partial row [2][D] of the weight gradients.
@@ -336,15 +364,15 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks)
                             T* __restrict__ dq, T* __restrict__ dk, float* __restrict__ partial, RopeParams p) {
   constexpr int kLanes = D / 8;
   const int l = lane_id() % kLanes;
-  float acc[2][8];
+  Four acc[2][2];      // of q and k: first and second members of the lane's pairs
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.f;
+  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = all4(0.f);
   wait_for_prior();
   const long warps = static_cast<long>(gridDim.x) * (kBwdThreads / 32), total = p.T * p.runs;
   for (long i = static_cast<long>(blockIdx.x) * (kBwdThreads / 32) + warp_id(); i < total; i += warps) {
     const long t = i / p.runs;
     const int h0 = static_cast<int>(i - t * p.runs) * p.run, h1 = min(h0 + p.run, p.Hq + p.Hk);
-    float c[4], s[4];
+    Four c, s;
     bool turned = false;
     if (h0 < p.Hq)
       backward_heads<T, D, INTER>(q + t * p.q_tok, p.q_head, dyq + t * p.dq_tok, p.dq_head, dq + t * p.oq_tok,
@@ -359,7 +387,8 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks)
   for (int side = 0; side < 2; ++side)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v = acc[side][i];
+      const float2 two = unpack2(acc[side][i >> 2].v[(i >> 1) & 1]);
+      float v = (i & 1) ? two.y : two.x;
 #pragma unroll
       for (int o = kLanes; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       const int pair = 4 * l + (i & 3), second = i >> 2;
