@@ -24,6 +24,9 @@ struct PackedItem {
   int q0, nq, k0, nk, diag, head, slot, pad;   // pad: parts of a split range; the second query tile's slot is slot + pad
 };
 constexpr int kItemInts = 8;
+// A batch all of whose items have at most this many query rows, and on average
+// kFewTiles key tiles or more, runs in the form for few rows over many keys.
+constexpr int kFewRows = 64, kFewTiles = 8;
 constexpr int kNoDiag = 1 << 29;   // bidirectional: every key is visible
 
 // Queries [q0, q0 + nq) of key/value head `head`, split into parts slot0 .. slot0 + parts - 1.
@@ -64,7 +67,7 @@ struct PackedBwdParams {
   KernelStatus status;
 };
 
-void launch_packed_fwd(int head_dim, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+void launch_packed_fwd(int head_dim, bool few, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                        const PackedFwdParams& p, cudaStream_t stream);
 void launch_packed_join(int head_dim, int joins, const PackedJoin* list, const PackedFwdParams& p,
                         cudaStream_t stream);

@@ -60,6 +60,7 @@ struct Fwd {
 
 struct Bars {
   uint64_t *q_full, *q_empty;
+  uint64_t *q_raw;       // a query tile with rows to be zeroed arrived (before q_full, see clean_warp)
   uint64_t *s_full;      // [t] S_t is in TMEM
   uint64_t *s_taken;     // S is in its warpgroup's registers, the columns are free
   uint64_t *p_full;      // [t] P_t is in TMEM
@@ -74,6 +75,7 @@ struct TileWork {
   int n0, n1;      // key tiles of each
   int most, tail;  // key tiles loaded; live rows of the last one if it is cut short, else 0
   bool solo;       // one query tile: key tile 2 j + t is step j of warpgroup t, else key tile j
+  int clear;       // first query row to be zeroed (few live rows over many keys), else 0
   __device__ __forceinline__ int n(int t) const { return t == 0 ? n0 : n1; }
   __device__ __forceinline__ int key_tile(int t, int j) const { return solo ? 2 * j + t : j; }
 };
@@ -83,7 +85,8 @@ __device__ __forceinline__ int tiles_seen(const PackedItem& it, int first, int t
   return (seen + 127) >> 7;
 }
 
-__device__ __forceinline__ TileWork tile_work(const PackedItem& it, int bt) {
+template <bool FEW>
+__device__ __forceinline__ TileWork tile_work(const PackedItem& it, int bt, int G) {
   TileWork w;
   w.solo = it.nq <= bt;
   w.n0 = tiles_seen(it, 0, min(bt, it.nq));
@@ -95,10 +98,11 @@ __device__ __forceinline__ TileWork tile_work(const PackedItem& it, int bt) {
   }
   const int left = it.nk - (w.most - 1) * 128;
   w.tail = (w.most > 0 && left < 128) ? left : 0;
+  w.clear = FEW && w.solo && w.most > 0 && it.nq * G <= kFewRows ? it.nq * G : 0;
   return w;
 }
 
-template <int D>
+template <int D, bool FEW>
 __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                           const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kK>& rk,
                                           const Ring<Fwd<D>::kV>& rv, const Bars& b, volatile int* abort_flag, const Slice& own) {
@@ -107,19 +111,22 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorM
   const uint32_t q_bytes = static_cast<uint32_t>(p.bt * p.G) * 128u * C::kChunks;
   Feed<C::kK> fk;
   Feed<C::kV> fv;
-  int q_used[2] = {0, 0};
-  bool ok = true;
+  int q_used[2] = {0, 0}, raws = 0;
+  bool ok = true, last_raw = false;
   for (int i = own.begin; i < own.end && ok; ++i) {
     const PackedItem it = own.item(p, i);
-    const TileWork w = tile_work(it, p.bt);
+    const TileWork w = tile_work<FEW>(it, p.bt, p.G);
     auto load_q = [&](int t) {
       if (w.n(t) == 0 || (w.solo && t == 1)) return true;
       if (!mbar_wait(&b.q_empty[t], (q_used[t] & 1) ^ 1u, limit, abort_flag)) return false;
       ++q_used[t];
-      mbar_arrive_expect_tx(&b.q_full[t], q_bytes);
+      uint64_t* full = w.clear != 0 ? b.q_raw : &b.q_full[t];
+      last_raw = w.clear != 0;
+      raws += w.clear != 0;
+      mbar_arrive_expect_tx(full, q_bytes);
 #pragma unroll
       for (int c = 0; c < C::kChunks; ++c)
-        tma_load_4d(sQ + t * C::kTile + c * kChunkBytes, &tq, &b.q_full[t], c * 64, 0, it.head, it.q0 + t * p.bt);
+        tma_load_4d(sQ + t * C::kTile + c * kChunkBytes, &tq, full, c * 64, 0, it.head, it.q0 + t * p.bt);
       return true;
     };
     ok = load_q(0);
@@ -148,12 +155,14 @@ __device__ __forceinline__ void load_warp(const CUtensorMap& tq, const CUtensorM
   fk.drain(rk, limit);
   fv.drain(rv, limit);
   volatile int never = 0;
-  for (int t = 0; t < 2; ++t)
+  // A raw tile becomes full by the cleaning warp's arrival, which a launch that gave up may never see.
+  if (last_raw) mbar_wait(b.q_raw, (raws - 1) & 1, limit, &never);
+  for (int t = last_raw ? 1 : 0; t < 2; ++t)
     if (q_used[t] > 0) mbar_wait(&b.q_full[t], (q_used[t] - 1) & 1, limit, &never);
 }
 
 // All scores, in the order (key tile, warpgroup).
-template <int D>
+template <int D, bool FEW>
 __device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kK>& rk, const Bars& b,
                                            volatile int* abort_flag, const Slice& own, uint32_t tmem) {
   using C = Fwd<D>;
@@ -164,7 +173,7 @@ __device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ
   uint32_t q_used0 = 0, q_used1 = 0, issued = 0;
   bool ok = true;
   for (int i = own.begin; i < own.end && ok; ++i) {
-    const TileWork w = tile_work(own.item(p, i), p.bt);
+    const TileWork w = tile_work<FEW>(own.item(p, i), p.bt, p.G);
     for (int kt = 0; kt < w.most && ok; ++kt, k.next()) {
       ok = mbar_wait(&rk.full[k.slot], k.phase, limit, abort_flag);
 #pragma unroll
@@ -199,7 +208,7 @@ __device__ __forceinline__ void score_warp(const PackedFwdParams& p, uint8_t* sQ
 }
 
 // All products with V, in the same order.
-template <int D>
+template <int D, bool FEW>
 __device__ __forceinline__ void value_warp(const PackedFwdParams& p, const Ring<Fwd<D>::kV>& rv, const Bars& b,
                                            volatile int* abort_flag, const Slice& own, uint32_t tmem) {
   using C = Fwd<D>;
@@ -210,7 +219,7 @@ __device__ __forceinline__ void value_warp(const PackedFwdParams& p, const Ring<
   uint32_t steps0 = 0, steps1 = 0;
   bool ok = true;
   for (int i = own.begin; i < own.end && ok; ++i) {
-    const TileWork w = tile_work(own.item(p, i), p.bt);
+    const TileWork w = tile_work<FEW>(own.item(p, i), p.bt, p.G);
     for (int kt = 0; kt < w.most && ok; ++kt, v.next()) {
       ok = mbar_wait(&rv.full[v.slot], v.phase, limit, abort_flag);
 #pragma unroll
@@ -235,15 +244,36 @@ __device__ __forceinline__ void value_warp(const PackedFwdParams& p, const Ring<
   finish_issuer(&b.drain[1], steps0 + steps1 > 0, ok, static_cast<int>(steps0 + steps1), p.status, abort_flag);
 }
 
-// Zeroes the rows past the sequence in the last V tile of each item that has such rows.
-template <int D>
-__device__ __forceinline__ void clean_warp(const PackedFwdParams& p, const Ring<Fwd<D>::kV>& rv,
+// Zeroes the rows past the sequence in the last V tile of each item that has
+// such rows, and (FEW) the query rows that nothing is asked of.  FEW is the form for single
+// new tokens over long keys (packed.h, kFewRows): bound by memory, but products of 124 foreign
+// rows and their exponentials took the GPU to its power cap and the clock to
+// 1.38 GHz.  With zeros there and their softmax warps idle (12 tokens over 151,000 keys, 32 heads
+// on 8, a sustained pass): 114.6 -> 109.5 us.  A form of its own, because the code for it in the
+// other one's loop cost short prompts 4 %.
+template <int D, bool FEW>
+__device__ __forceinline__ void clean_warp(const PackedFwdParams& p, uint8_t* sQ, const Ring<Fwd<D>::kV>& rv, const Bars& b,
                                            volatile int* abort_flag, const Slice& own) {
   using C = Fwd<D>;
-  int base = 0;
+  int base = 0, raws = 0;
   uint32_t parity = 0;
   for (int i = own.begin; i < own.end; ++i) {
-    const TileWork w = tile_work(own.item(p, i), p.bt);
+    const TileWork w = tile_work<FEW>(own.item(p, i), p.bt, p.G);
+    if (w.clear != 0) {
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(b.q_raw, raws & 1, p.status.limit_ns, abort_flag));
+      if (!ok) {
+        if (lane_id() == 0) {
+          report_status(p.status, kStatusTimeoutFull, i);
+          *abort_flag = 1;
+        }
+        return;
+      }
+      ++raws;
+      zero_tile_rows<C::kChunks>(sQ, w.clear);
+      fence_async_smem();
+      __syncwarp();
+      if (lane_id() == 0) mbar_arrive(&b.q_full[0]);
+    }
     if (w.tail != 0 &&
         !clean_tile<C::kChunks, C::kTile>(rv, base + w.most - 1, w.tail, parity, p.status.limit_ns, abort_flag)) {
       if (lane_id() == 0) {
@@ -290,7 +320,27 @@ __device__ __forceinline__ float row_exp(uint32_t (&r)[4][32], float scale, floa
   return a + b;
 }
 
-template <int D>
+// The turns of a warp without a live row: P is zero.
+__device__ __forceinline__ bool pass_on(uint64_t* s_full, uint64_t* s_taken, uint64_t* p_full, uint64_t* pv_done, uint32_t tP,
+                                     int steps, int n_kv, uint64_t limit, volatile int* abort_flag) {
+  for (int j = 0; j < n_kv; ++j, ++steps) {
+    if (!__all_sync(0xffffffffu, mbar_wait(s_full, steps & 1, limit, abort_flag))) return false;
+    warp_arrive(s_taken);
+    if (j == 0) {
+      const uint32_t zeros[16] = {};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_st16(tP + c * 16, zeros);
+      tmem_st_wait();
+      tc_fence_before();
+    } else if (!__all_sync(0xffffffffu, mbar_wait(pv_done, (steps - 1) & 1, limit, abort_flag))) {
+      return false;
+    }
+    warp_arrive(p_full);
+  }
+  return true;
+}
+
+template <int D, bool FEW>
 __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Bars& b, volatile int* abort_flag, const Slice& own,
                                               float2* exchange, uint32_t tmem, int t) {
   const uint64_t limit = p.status.limit_ns;
@@ -303,16 +353,22 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
   bool ok = true;
   for (int i = own.begin; i < own.end; ++i) {
     const PackedItem it = own.item(p, i);
-    const TileWork w = tile_work(it, p.bt);
+    const TileWork w = tile_work<FEW>(it, p.bt, p.G);
     const int first = w.solo ? 0 : t * p.bt, n_kv = w.n(t);
     other_steps += w.n(t ^ 1);
     const bool both = w.solo && w.n1 > 0;      // one query tile, both warpgroups on it
     if (w.solo ? t == 1 && !both : it.nq <= first) continue;
     const bool live = row < min(p.bt, it.nq - first) * p.G;
+    const bool idle = FEW && w.clear != 0 && (warp_id() & 3) * 32 >= w.clear;
     // Keys that this row sees; rows that are not stored see every key of the item.
     const int seen = live ? min(it.nk, max(0, first + tok + it.diag + 1)) : it.nk;
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < n_kv; ++j, ++steps) {
+    // Few rows over many keys: a warp without a live row only passes the turns on, its P is zero for the whole item.
+    if (idle) {
+      ok = pass_on(b.s_full + t, b.s_taken, b.p_full + t, b.pv_done + t, tP, steps, n_kv, limit, abort_flag);
+      steps += n_kv;
+    }
+    for (int j = 0; !idle && j < n_kv; ++j, ++steps) {
       // Warp-uniform outcome: tcgen05.ld/st below are warp-collective.
       ok = __all_sync(0xffffffffu, mbar_wait(&b.s_full[t], steps & 1, limit, abort_flag));
       if (!ok) break;
@@ -463,7 +519,7 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
   }
 }
 
-template <int D>
+template <int D, bool FEW>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ PackedFwdParams p) {
@@ -484,9 +540,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   b.s_taken = bars + 12;
   b.traded = bars + 13;
   b.joined = bars + 15;
-  rk.place(bars + 17, sQ + 2 * C::kTile);
-  rv.place(bars + 17 + rk.kBarriers, rk.base + C::kK * C::kTile);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17 + rk.kBarriers + rv.kBarriers);
+  b.q_raw = bars + 17;
+  rk.place(bars + 18, sQ + 2 * C::kTile);
+  rv.place(bars + 18 + rk.kBarriers, rk.base + C::kK * C::kTile);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18 + rk.kBarriers + rv.kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id();
   const Slice own(p.items, p.begin);
@@ -505,6 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&b.drain[0], 1);
     mbar_init(&b.drain[1], 1);
     mbar_init(b.s_taken, 4);
+    mbar_init(b.q_raw, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tq);
@@ -523,13 +581,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     setmaxnreg_dec<kRegsLow>();
     if (warp == 0) {
-      if (elect_one()) load_warp<D>(tq, tk, tv, p, sQ, rk, rv, b, abort_flag, own);
+      if (elect_one()) load_warp<D, FEW>(tq, tk, tv, p, sQ, rk, rv, b, abort_flag, own);
     } else if (warp == 1) {
-      if (elect_one()) score_warp<D>(p, sQ, rk, b, abort_flag, own, tmem);
+      if (elect_one()) score_warp<D, FEW>(p, sQ, rk, b, abort_flag, own, tmem);
     } else if (warp == 2) {
-      clean_warp<D>(p, rv, abort_flag, own);
+      clean_warp<D, FEW>(p, sQ, rv, b, abort_flag, own);
     } else {
-      if (elect_one()) value_warp<D>(p, rv, b, abort_flag, own, tmem);
+      if (elect_one()) value_warp<D, FEW>(p, rv, b, abort_flag, own, tmem);
     }
     __syncwarp();
     tc_fence_before();
@@ -541,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   setmaxnreg_inc<kRegsHigh>();
-  softmax_warps<D>(p, b, abort_flag, own, exchange, tmem, (warp - 4) >> 2);
+  softmax_warps<D, FEW>(p, b, abort_flag, own, exchange, tmem, (warp - 4) >> 2);
   __syncwarp();
   tc_fence_before();
   named_bar_sync(1, kThreads);
@@ -616,18 +674,12 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const PackedJoin* __re
   }
 }
 
-template <int D>
-void fwd(int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const PackedFwdParams& p,
-         cudaStream_t stream) {
-  launch_overlapped(packed_fwd_kernel<D>, blocks, kThreads, Fwd<D>::kSmem, stream, q, k, v, p);
-}
-
-template <int D>
+template <int D, bool FEW>
 const char* configure() {
   cudaFuncAttributes attr{};
-  if (cudaFuncSetAttribute(packed_fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fwd<D>::kSmem) !=
+  if (cudaFuncSetAttribute(packed_fwd_kernel<D, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fwd<D>::kSmem) !=
           cudaSuccess ||
-      cudaFuncGetAttributes(&attr, packed_fwd_kernel<D>) != cudaSuccess)
+      cudaFuncGetAttributes(&attr, packed_fwd_kernel<D, FEW>) != cudaSuccess)
     return "cannot configure the packed attention forward kernel";
   // setmaxnreg.inc waits for registers that the producer warpgroup releases:
   // it only balances if the launch count is the assumed one.
@@ -638,14 +690,16 @@ const char* configure() {
 }  // namespace
 
 const char* packed_fwd_configure() {
-  const char* e = configure<64>();
-  return e != nullptr ? e : configure<128>();
+  for (const char* e : {configure<64, false>(), configure<64, true>(), configure<128, false>(), configure<128, true>()})
+    if (e != nullptr) return e;
+  return nullptr;
 }
 
-void launch_packed_fwd(int head_dim, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                       const PackedFwdParams& p, cudaStream_t stream) {
-  if (head_dim == 128) fwd<128>(blocks, q, k, v, p, stream);
-  else fwd<64>(blocks, q, k, v, p, stream);
+void launch_packed_fwd(int head_dim, bool few, int blocks, const CUtensorMap& q, const CUtensorMap& k,
+                       const CUtensorMap& v, const PackedFwdParams& p, cudaStream_t stream) {
+  auto go = [&](auto kernel, int smem) { launch_overlapped(kernel, blocks, kThreads, smem, stream, q, k, v, p); };
+  if (head_dim == 128) go(few ? packed_fwd_kernel<128, true> : packed_fwd_kernel<128, false>, Fwd<128>::kSmem);
+  else go(few ? packed_fwd_kernel<64, true> : packed_fwd_kernel<64, false>, Fwd<64>::kSmem);
 }
 
 void launch_packed_join(int head_dim, int joins, const PackedJoin* list, const PackedFwdParams& p,

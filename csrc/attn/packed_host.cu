@@ -33,7 +33,7 @@ constexpr double kJoinCost = 4.0;
 
 enum Meta : int {
   kTq, kTk, kHq, kHk, kD, kFwdItems, kFwdBegin, kFwdBlocks, kJoins, kJoinCount, kSlots, kPartRows,
-  kDqItems, kDqBegin, kDqBlocks, kDkvItems, kDkvBegin, kDkvBlocks, kBlobInts, kMetaCount
+  kDqItems, kDqBegin, kDqBlocks, kDkvItems, kDkvBegin, kDkvBlocks, kBlobInts, kFew, kMetaCount
 };
 
 struct Costed {
@@ -388,6 +388,12 @@ std::tuple<at::Tensor, std::vector<int64_t>> packed_schedule(const std::vector<i
   int most = 0;
   for (const Costed& c : fwd) most = std::max(most, c.tiles);
   if (most >= 2 * kMinPart) cut = cut_evenly(fwd, kv_heads, n_sms, bt, group);
+  int64_t key_tiles = 0, most_rows = 0;
+  for (const Costed& c : fwd) {
+    key_tiles += c.tiles;
+    most_rows = std::max<int64_t>(most_rows, static_cast<int64_t>(c.item.nq) * group);
+  }
+  meta[kFew] = !fwd.empty() && most_rows <= kFewRows && key_tiles >= kFewTiles * static_cast<int64_t>(fwd.size());
   const bool use_cut = !cut.joins.empty() && cut.bins.makespan + kJoinCost < whole.makespan;
   const Bins& chosen = use_cut ? cut.bins : whole;
   blob.add_bins(chosen, meta[kFwdItems], meta[kFwdBegin]);
@@ -455,7 +461,7 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q_in, const at::T
     p.part_extent = rows * head_dim;
   }
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
-  launch_packed_fwd(head_dim, static_cast<int>(meta[kFwdBlocks]), query_map(q, p.G, p.bt), key_map(k), key_map(v), p,
+  launch_packed_fwd(head_dim, meta[kFew] != 0, static_cast<int>(meta[kFwdBlocks]), query_map(q, p.G, p.bt), key_map(k), key_map(v), p,
                     stream);
   after_launch();
   if (meta[kJoinCount] > 0) {

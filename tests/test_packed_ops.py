@@ -328,6 +328,8 @@ ATTENTION = [
     ([5, 140, 3], [0, 20, 0], 2, 1, True), ([0, 9], [200, 0], 2, 2, False),
     # key ranges that are split over blocks
     ([1, 2], [9000, 5000], 8, 2, True), ([400], [6000], 2, 2, False), ([2, 300], [7000, 4100], 7, 1, True),
+    # few rows over many keys, some sequences without keys or queries
+    ([1, 3, 0, 2], [9000, 0, 77, 6000], 8, 2, True), ([1, 1], [5000, 3001], 4, 4, False), ([9], [4000], 14, 2, True),
 ]
 
 
