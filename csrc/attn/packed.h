@@ -21,7 +21,8 @@ namespace h3 {
 //                 iff j <= i + diag; slot >= 0: a part of a split key range, result to the partial buffers
 //   dk / dv     : keys [k0, k0 + nk) (one tile) against queries [q0, q0 + nq), same diag rule
 struct PackedItem {
-  int q0, nq, k0, nk, diag, head, slot, pad;   // pad: parts of a split range; the second query tile's slot is slot + pad
+  int q0, nq, k0, nk, diag, head, slot;
+  int pad;   // parts of a split range; the second query tile's slot is slot + pad
 };
 constexpr int kItemInts = 8;
 // A batch all of whose items have at most this many query rows, and on average
@@ -67,8 +68,8 @@ struct PackedBwdParams {
   KernelStatus status;
 };
 
-void launch_packed_fwd(int head_dim, bool few, int blocks, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                       const PackedFwdParams& p, cudaStream_t stream);
+void launch_packed_fwd(int head_dim, bool few, int blocks, const CUtensorMap& q, const CUtensorMap& k,
+                       const CUtensorMap& v, const PackedFwdParams& p, cudaStream_t stream);
 void launch_packed_join(int head_dim, int joins, const PackedJoin* list, const PackedFwdParams& p,
                         cudaStream_t stream);
 void launch_packed_delta(int head_dim, const PackedBwdParams& p, cudaStream_t stream);

@@ -181,8 +181,8 @@ Cut cut_evenly(const std::vector<Costed>& one_head, int64_t kv_heads, int sms, i
 }
 
 int key_tiles_of(const PackedItem& it) {
-  return static_cast<int>((std::min<int64_t>(it.nk, std::max<int64_t>(0, static_cast<int64_t>(it.nq) + it.diag)) + 127) /
-                          128);
+  const int64_t seen = std::min<int64_t>(it.nk, std::max<int64_t>(0, static_cast<int64_t>(it.nq) + it.diag));
+  return static_cast<int>((seen + 127) / 128);
 }
 
 // Sections of the blob start on 32-byte boundaries.
@@ -461,8 +461,8 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q_in, const at::T
     p.part_extent = rows * head_dim;
   }
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
-  launch_packed_fwd(head_dim, meta[kFew] != 0, static_cast<int>(meta[kFwdBlocks]), query_map(q, p.G, p.bt), key_map(k), key_map(v), p,
-                    stream);
+  launch_packed_fwd(head_dim, meta[kFew] != 0, static_cast<int>(meta[kFwdBlocks]), query_map(q, p.G, p.bt),
+                    key_map(k), key_map(v), p, stream);
   after_launch();
   if (meta[kJoinCount] > 0) {
     launch_packed_join(head_dim, static_cast<int>(meta[kJoinCount]),

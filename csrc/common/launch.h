@@ -9,10 +9,11 @@ void note_launch();
 #ifdef __CUDACC__
 // A kernel launched this way may be resident before the stream's previous
 // kernel has ended; it must call wait_for_prior() in every thread before it
-// touches memory that earlier work reads or writes.  The set-up before that call (barriers, TMEM,
-// the work list) then costs nothing between kernels.
+// touches memory that earlier work reads or writes.  The set-up before that call
+// (barriers, TMEM, the work list) then costs nothing between kernels.
 template <typename... P, typename... A>
-inline void launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+inline void launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                              A&&... args) {
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;

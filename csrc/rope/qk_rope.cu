@@ -16,6 +16,9 @@
 // group, x is never read twice, there are no [T, D/2] tables, no shared memory
 // and no barriers.  The loads of the next batch of heads are issued before the
 // current batch is worked on.
+// Measured (37,730 tokens, 42 + 42 heads of 128, bf16, 1.62 GB): rotation 257 us =
+// 6.3 TB/s, with norms 264 us in a burst and 267 us under the power cap; gradients of
+// 16,411 tokens, 32 + 8 heads (504 MB) 93 us = 5.4 TB/s.
 // The weight gradients stay in registers over all tokens of a warp (a lane's
 // columns are fixed) and are summed in a fixed order: per block into a partial
 // row, and by a second small kernel over the rows.
@@ -632,10 +635,10 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
     const long blocks = (p.T * p.runs + kBwdThreads / 32 - 1) / (kBwdThreads / 32);
     const int grid = static_cast<int>(std::min<long>(blocks, resident_blocks(kernel, kBwdThreads)));
     auto partial = empty_cuda({grid, 2 * kD}, at::kFloat, q);
-    launch_overlapped(
-        kernel, grid, kBwdThreads, 0, stream, reinterpret_cast<const T*>(q.data_ptr()), reinterpret_cast<const T*>(k.data_ptr()), qw, kw,
-        reinterpret_cast<const T*>(dq_out.data_ptr()), reinterpret_cast<const T*>(dk_out.data_ptr()),
-        reinterpret_cast<T*>(dq.data_ptr()), reinterpret_cast<T*>(dk.data_ptr()), partial.data_ptr<float>(), p);
+    launch_overlapped(kernel, grid, kBwdThreads, 0, stream, reinterpret_cast<const T*>(q.data_ptr()),
+                      reinterpret_cast<const T*>(k.data_ptr()), qw, kw, reinterpret_cast<const T*>(dq_out.data_ptr()),
+                      reinterpret_cast<const T*>(dk_out.data_ptr()), reinterpret_cast<T*>(dq.data_ptr()),
+                      reinterpret_cast<T*>(dk.data_ptr()), partial.data_ptr<float>(), p);
     note_launch();
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     launch_overlapped(sum_partials_kernel, 2 * kD / 32, dim3(32, 32), 0, stream, partial.data_ptr<float>(), grid, kD,

@@ -448,7 +448,7 @@ def test_attention_layouts(K):
     o, lse = K.attention_packed_fwd(q, k, v, plan)
     assert torch.equal(o, want_o) and torch.equal(lse, want_lse)
     want = K.attention_packed_bwd(q.contiguous(), k.contiguous(), v.contiguous(), o, lse, do.contiguous(), plan)
-    fused = torch.full((135, 9 * 64), 7.0, dtype=torch.bfloat16, device="cuda")     # dq, dk, dv and a spare column block
+    fused = torch.full((135, 9 * 64), 7.0, dtype=torch.bfloat16, device="cuda")     # and a spare block of columns
     out = fused[:, :256].view(135, 4, 64), fused[:, 256:384].view(135, 2, 64), fused[:, 384:512].view(135, 2, 64)
     got = K.attention_packed_bwd(q, k, v, o, lse, do, plan, out=out)
     for a, b, c in zip(got, want, out):
@@ -524,7 +524,8 @@ def test_out_views_and_their_refusals(K):
     got = K.qk_norm_rope_bwd(q, k, w, w, rope, dq, dk, out=out)
     assert got[0].data_ptr() == out[0].data_ptr() and all(torch.equal(a, b) for a, b in zip(got, want))
     assert (fused[:, 384:] == 7.0).all()
-    for bad, message in (((out[0],), "dq and dk"), ((out[0], out[0]), "heads of q and k"), ((out[0].float(), out[1]), "type"),
+    for bad, message in (((out[0],), "dq and dk"), ((out[0], out[0]), "heads of q and k"),
+                         ((out[0].float(), out[1]), "type"),
                          ((fused[:, 1:257].view(50, 4, 64), out[1]), "16-byte")):
         with pytest.raises(RuntimeError, match=message):
             K.qk_norm_rope_bwd(q, k, w, w, rope, dq, dk, out=bad)
@@ -541,7 +542,8 @@ def test_checked_build_agrees(K):
 
     checked = NativeKernels(torch.device("cuda", 0), wait_limit_s=2.0, extension=_C_checked)
     torch.manual_seed(15)
-    for q_lens, k_lens, heads, kv, dim, causal in (([77, 1, 300], None, 6, 2, 128, True), ([1, 2], [9000, 400], 8, 2, 64, True)):
+    for q_lens, k_lens, heads, kv, dim, causal in (([77, 1, 300], None, 6, 2, 128, True),
+                                                   ([1, 2], [9000, 400], 8, 2, 64, True)):
         plan = K.packed_plan(q_lens, k_lens, heads=heads, kv_heads=kv, head_dim=dim, causal=causal)
         q, k, v = make(plan)
         do = bf(plan.q_tokens, heads, dim)

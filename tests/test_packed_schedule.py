@@ -43,7 +43,8 @@ def _expected(q_lens, k_lens, causal):
 CASES = [
     ([5], None, 1, 1, True), ([128, 1, 0, 77], None, 8, 2, True), ([300, 20], [300, 20], 6, 2, False),
     ([1, 1, 1], [1500, 3, 700], 8, 2, True), ([1], [6000], 4, 4, False), ([9, 200], [4, 100], 3, 3, True),
-    ([0, 0], [10, 300], 2, 1, True), ([700], [0], 2, 2, False), ([1300], None, 7, 1, True), ([64, 64], None, 256, 2, False),
+    ([0, 0], [10, 300], 2, 1, True), ([700], [0], 2, 2, False), ([1300], None, 7, 1, True),
+    ([64, 64], None, 256, 2, False),
 ]
 
 
