@@ -47,18 +47,36 @@ struct Bins {
   double makespan = 0.0;
 };
 
-// Items to the least loaded block, in the given order.
-Bins deal(const std::vector<Costed>& items, int sms) {
+// An item of one head's list for one head.
+struct Pick {
+  int item, head;
+};
+
+// Picks to the least loaded block, in the given order.
+Bins deal(const std::vector<Costed>& one_head, const std::vector<Pick>& order, int sms) {
   Bins bins;
-  const int n = static_cast<int>(std::min<size_t>(sms, items.size()));
+  const int n = static_cast<int>(std::min<size_t>(sms, order.size()));
   bins.of.resize(n);
+  for (auto& b : bins.of) b.reserve(order.size() / std::max(n, 1) + 2);
+  const bool level = one_head.front().cost == one_head.back().cost;      // sorted: all cost the same
+  if (level) {
+    for (size_t i = 0; i < order.size(); ++i) {
+      bins.of[i % n].push_back(one_head[order[i].item].item);
+      bins.of[i % n].back().head = order[i].head;
+    }
+    bins.makespan = one_head.front().cost * static_cast<double>((order.size() + n - 1) / n);
+    return bins;
+  }
   using Load = std::pair<double, int>;
-  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
-  for (int i = 0; i < n; ++i) least.emplace(0.0, i);
-  for (const Costed& c : items) {
+  std::vector<Load> start;
+  for (int i = 0; i < n; ++i) start.emplace_back(0.0, i);
+  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least(std::greater<Load>(), std::move(start));
+  for (const Pick& pick : order) {
     Load l = least.top();
     least.pop();
+    const Costed& c = one_head[pick.item];
     bins.of[l.second].push_back(c.item);
+    bins.of[l.second].back().head = pick.head;
     l.first += c.cost;
     bins.makespan = std::max(bins.makespan, l.first);
     least.push(l);
@@ -72,21 +90,22 @@ Bins deal(const std::vector<Costed>& items, int sms) {
 // heads: the longest block 45 % over the mean); then longest first over all
 // heads, unless it gains less than 5 %.
 Bins balance(std::vector<Costed> one_head, int64_t kv_heads, int sms) {
-  auto longer = [](const Costed& a, const Costed& b) { return a.cost > b.cost; };
-  std::stable_sort(one_head.begin(), one_head.end(), longer);
-  std::vector<Costed> all;
-  all.reserve(one_head.size() * kv_heads);
-  for (int64_t h = 0; h < kv_heads; ++h)
-    for (Costed c : one_head) {
-      c.item.head = static_cast<int>(h);
-      all.push_back(c);
-    }
-  Bins by_head = deal(all, sms);
+  if (one_head.empty()) return Bins();
+  std::stable_sort(one_head.begin(), one_head.end(), [](const Costed& a, const Costed& b) { return a.cost > b.cost; });
   double total = 0.0;
-  for (const Costed& c : all) total += c.cost;
-  if (by_head.makespan * sms <= 1.05 * total) return by_head;
-  std::stable_sort(all.begin(), all.end(), longer);
-  Bins mixed = deal(all, sms);
+  for (const Costed& c : one_head) total += c.cost;
+  total *= static_cast<double>(kv_heads);
+  const int items = static_cast<int>(one_head.size()), heads = static_cast<int>(kv_heads);
+  std::vector<Pick> order;
+  order.reserve(static_cast<size_t>(items) * heads);
+  for (int h = 0; h < heads; ++h)
+    for (int i = 0; i < items; ++i) order.push_back({i, h});
+  Bins by_head = deal(one_head, order, sms);
+  if (by_head.makespan * sms <= 1.05 * total || one_head.front().cost == one_head.back().cost) return by_head;
+  order.clear();
+  for (int i = 0; i < items; ++i)       // the list is sorted: the same item of every head in a row
+    for (int h = 0; h < heads; ++h) order.push_back({i, h});
+  Bins mixed = deal(one_head, order, sms);
   return mixed.makespan * 1.05 < by_head.makespan ? mixed : by_head;
 }
 
@@ -99,20 +118,15 @@ struct Cut {
 };
 
 // One walk with blocks of `share` steps; false if they do not hold all items.
-bool cut_into(const std::vector<Costed>& one_head, int64_t kv_heads, int sms, int bt, int group, double share,
-              Cut& out) {
-  out = Cut();
-  out.bins.of.resize(sms);
+// Calls piece(item's index, head, block, first tile, last tile + 1) for each piece, an item's pieces in a row.
+template <typename F>
+bool walk(const std::vector<Costed>& one_head, int64_t kv_heads, int sms, double share, F&& piece) {
   int block = 0;
   double left = share;
-  struct Piece {
-    int block, from, to;
-  };
   for (int64_t h = 0; h < kv_heads; ++h)
-    for (const Costed& c : one_head) {
-      std::vector<Piece> pieces;
+    for (size_t n = 0; n < one_head.size(); ++n) {
+      const int tiles = one_head[n].tiles;
       int from = 0;
-      const int tiles = c.tiles;
       for (;;) {
         const int rest = tiles - from;
         int take = rest;
@@ -130,54 +144,73 @@ bool cut_into(const std::vector<Costed>& one_head, int64_t kv_heads, int sms, in
           }
         }
         if (block >= sms) return false;
-        pieces.push_back({block, from, from + take});
+        piece(n, h, block, from, from + take);
         left -= take + kItemCost;
         from += take;
         if (from >= tiles) break;
         ++block;
         left = share;
       }
-      const int tiles_q = (c.item.nq + bt - 1) / bt, parts = static_cast<int>(pieces.size());
-      for (int i = 0; i < parts; ++i) {
-        PackedItem item = c.item;
-        item.head = static_cast<int>(h);
-        if (parts > 1) {
-          item.k0 += pieces[i].from * 128;
-          item.nk = std::min(item.nk, pieces[i].to * 128) - pieces[i].from * 128;
-          item.diag = item.diag == kNoDiag ? kNoDiag : item.diag - pieces[i].from * 128;
-          item.slot = out.slots + i;
-          item.pad = parts;      // the second query tile's parts follow the first's
-        }
-        out.bins.of[pieces[i].block].push_back(item);
-      }
-      if (parts > 1) {
-        for (int t = 0; t < tiles_q; ++t) {
-          const int tokens = std::min(bt, c.item.nq - t * bt);
-          out.joins.push_back({c.item.q0 + t * bt, tokens, static_cast<int>(h), out.slots + t * parts, parts, 0, 0, 0});
-          out.part_rows = std::max(out.part_rows, tokens * group);
-        }
-        out.slots += parts * tiles_q;
-      }
     }
-  for (const auto& b : out.bins.of) {
-    double load = 0.0;
-    for (const PackedItem& it : b) load += (std::min(it.nk, std::max(0, it.nq + it.diag)) + 127) / 128 + kItemCost;
-    out.bins.makespan = std::max(out.bins.makespan, load);
-  }
-  out.bins.of.erase(std::remove_if(out.bins.of.begin(), out.bins.of.end(), [](const auto& b) { return b.empty(); }),
-                    out.bins.of.end());
   return true;
 }
 
 // The smallest share (in steps of 3 %) that holds everything: pieces cost more than the items they come from.
 Cut cut_evenly(const std::vector<Costed>& one_head, int64_t kv_heads, int sms, int bt, int group) {
+  struct Piece {
+    size_t item;
+    int64_t head;
+    int block, from, to;
+  };
   double total = 0.0;
   for (const Costed& c : one_head) total += c.tiles + kItemCost;
   double share = std::max(kMinPart + kItemCost, total * static_cast<double>(kv_heads) / sms);
+  auto nothing = [](size_t, int64_t, int, int, int) {};
+  int tries = 0;
+  while (!walk(one_head, kv_heads, sms, share, nothing)) {
+    if (++tries == 48) return Cut();
+    share = share * 1.03 + 0.25;
+  }
+  std::vector<Piece> pieces;
+  walk(one_head, kv_heads, sms, share, [&](size_t n, int64_t h, int block, int from, int to) {
+    pieces.push_back({n, h, block, from, to});
+  });
   Cut out;
-  for (int tries = 0; tries < 48; ++tries, share = share * 1.03 + 0.25)
-    if (cut_into(one_head, kv_heads, sms, bt, group, share, out)) return out;
-  return Cut();
+  out.bins.of.resize(sms);
+  std::vector<double> loads(sms, 0.0);
+  for (size_t i = 0; i < pieces.size();) {
+    size_t end = i + 1;
+    while (end < pieces.size() && pieces[end].item == pieces[i].item && pieces[end].head == pieces[i].head) ++end;
+    const PackedItem& whole = one_head[pieces[i].item].item;
+    const int tiles_q = (whole.nq + bt - 1) / bt, parts = static_cast<int>(end - i);
+    for (size_t k = i; k < end; ++k) {
+      PackedItem item = whole;
+      item.head = static_cast<int>(pieces[k].head);
+      if (parts > 1) {
+        item.k0 += pieces[k].from * 128;
+        item.nk = std::min(item.nk, pieces[k].to * 128) - pieces[k].from * 128;
+        item.diag = item.diag == kNoDiag ? kNoDiag : item.diag - pieces[k].from * 128;
+        item.slot = out.slots + static_cast<int>(k - i);
+        item.pad = parts;      // the second query tile's parts follow the first's
+      }
+      out.bins.of[pieces[k].block].push_back(item);
+      loads[pieces[k].block] += pieces[k].to - pieces[k].from + kItemCost;
+    }
+    if (parts > 1) {
+      for (int t = 0; t < tiles_q; ++t) {
+        const int tokens = std::min(bt, whole.nq - t * bt);
+        out.joins.push_back({whole.q0 + t * bt, tokens, static_cast<int>(pieces[i].head), out.slots + t * parts, parts,
+                             0, 0, 0});
+        out.part_rows = std::max(out.part_rows, tokens * group);
+      }
+      out.slots += parts * tiles_q;
+    }
+    i = end;
+  }
+  out.bins.makespan = *std::max_element(loads.begin(), loads.end());
+  out.bins.of.erase(std::remove_if(out.bins.of.begin(), out.bins.of.end(), [](const auto& b) { return b.empty(); }),
+                    out.bins.of.end());
+  return out;
 }
 
 int key_tiles_of(const PackedItem& it) {
@@ -387,7 +420,11 @@ std::tuple<at::Tensor, std::vector<int64_t>> packed_schedule(const std::vector<i
   Cut cut;
   int most = 0;
   for (const Costed& c : fwd) most = std::max(most, c.tiles);
-  if (most >= 2 * kMinPart) cut = cut_evenly(fwd, kv_heads, n_sms, bt, group);
+  double total = 0.0;
+  for (const Costed& c : fwd) total += c.cost * static_cast<double>(kv_heads);
+  // No cutting levels better than the mean.
+  if (most >= 2 * kMinPart && whole.makespan > total / n_sms + kJoinCost)
+    cut = cut_evenly(fwd, kv_heads, n_sms, bt, group);
   int64_t key_tiles = 0, most_rows = 0;
   for (const Costed& c : fwd) {
     key_tiles += c.tiles;
