@@ -219,7 +219,7 @@ class NativeKernels:
     def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6, out=None):
         """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32.
 
-        ``out``: two tensors (views are fine) to write dq and dk into.  The
+        ``out``: two tensors (views are fine, not over the inputs) to write dq and dk into.  The
         weights' sums run in a fixed order.
         """
         pos, freqs, pairs, inter = self._rope_args(rope)
@@ -250,7 +250,7 @@ class NativeKernels:
         return o, lse
 
     def attention_packed_bwd(self, q, k, v, o, lse, do, plan: PackedPlan, scale=None, out=None):
-        """Gradients ``(dq, dk, dv)``; ``out``: three tensors (views are fine) to write them into.
+        """Gradients ``(dq, dk, dv)``; ``out``: three tensors (views are fine, not over the inputs) to write them into.
 
         The sums over the heads of a group and over query tiles run in a fixed
         order: the same inputs give the same bits.

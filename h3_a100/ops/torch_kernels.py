@@ -266,7 +266,7 @@ class TorchKernels:
     def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6, out=None):
         """Gradients ``(dq, dk, dq_weight, dk_weight)`` from those of the outputs; the weights' in fp32.
 
-        ``out``: two tensors (views are fine) to write dq and dk into.
+        ``out``: two tensors (views are fine, not over the inputs) to write dq and dk into.
         """
         cos, sin = self._axis_tables(rope, q.shape[-1], q)
         grads, weights = [], []
