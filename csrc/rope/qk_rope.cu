@@ -341,14 +341,14 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
       // Both sums before r is known, so that their shuffles overlap.
       const float ss = group_sum<kLanes>(sum4(fma4(a, a, mul4(b, b))));
       const float gx = group_sum<kLanes>(sum4(fma4(gwa, a, mul4(gwb, b))));
-      // Rows past h1 are zeros: r is finite and everything below is zero.
-      const float r = rsqrtf(ss * (1.f / D) + p.eps);
+      // A place past h1 holds zeros and weighs nothing: without eps the r of its row would be infinite.
+      const int at = h + u * kGroups + g;
+      const float r = at < h1 ? rsqrtf(ss * (1.f / D) + p.eps) : 0.f;
       const Four r4 = all4(r), back = all4(-r * r * r * (gx * (1.f / D)));
       acc[0] = fma4(mul4(ga, r4), a, acc[0]);
       acc[1] = fma4(mul4(gb, r4), b, acc[1]);
       ya = fma4(a, back, mul4(gwa, r4));
       yb = fma4(b, back, mul4(gwb, r4));
-      const int at = h + u * kGroups + g;
       if (at < h1) store_pairs<D, INTER>(dx + at * dx_head, l, ya, yb);
     }
   }

@@ -1,0 +1,57 @@
+"""Packed-sequence operators at the edges of their range, against formulas in 64 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_packed_ops import K, U, bf, norm_turned, rope_of, turned  # noqa: F401  (K is a fixture)
+
+gpu = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- gradients of the norms
+def turned_size(x, rope):
+    """The sum of the absolute values of the two terms of every rotated element, in 64 bits."""
+    x = x.double()
+    a, b = torch.zeros_like(x), torch.zeros_like(x)
+    half = x.shape[-1] // 2
+    first = torch.arange(x.shape[-1]) % 2 == 0 if rope is None or rope.interleaved else torch.arange(x.shape[-1]) < half
+    a[..., first], b[..., ~first] = x[..., first], x[..., ~first]
+    return turned(a, rope).abs() + turned(b, rope).abs()
+
+
+def check_norm_gradients(K, q, k, qw, kw, rope, dq, dk, eps):
+    grads = K.qk_norm_rope_bwd(q, k, qw, kw, rope, dq, dk, eps=eps)
+    for x, w, dy, dx, dw in ((q, qw, dq, grads[0], grads[2]), (k, kw, dk, grads[1], grads[3])):
+        xd, wd = x.double().requires_grad_(True), w.double().requires_grad_(True)
+        want = torch.autograd.grad(norm_turned(xd, wd, rope, eps), (xd, wd), dy.double())
+        xd = xd.detach()
+        r = torch.rsqrt(xd.square().mean(-1, keepdim=True) + eps)
+        n, g = xd * r, turned(dy, rope, -1.0)
+        gw = g * w.double()
+        # fp32: about ten roundings and one reciprocal root (two units) of terms of this size, then the type's own
+        size = r * (gw.abs() + n.abs() * (gw * n).mean(-1, keepdim=True).abs()).amax(-1, keepdim=True)
+        bound = 2.0 ** -19 * size + (U * want[0].abs() if x.dtype == torch.bfloat16 else 0.0) + 1e-37
+        assert dx.dtype == x.dtype and ((dx.double() - want[0]).abs() <= bound).all()
+        # fp32 sums over tokens and heads of terms (dy0 cos + dy1 sin) n: 2^-22 of the sum of absolute values covers a
+        # tree of them
+        assert dw.dtype == torch.float32
+        assert ((dw.double() - want[1]).abs() <= 2.0 ** -18 * (turned_size(dy, rope) * n.abs()).sum((0, 1))).all()
+
+
+def norm_inputs(tokens, heads, kv_heads, dim, dtype, size=1.0):
+    return (bf(tokens, heads, dim, scale=size, dtype=dtype), bf(tokens, kv_heads, dim, scale=size, dtype=dtype),
+            1 + 0.3 * bf(dim, dtype=torch.float32), bf(dim, dtype=torch.float32),
+            bf(tokens, heads, dim, dtype=dtype), bf(tokens, kv_heads, dim, scale=3.0, dtype=dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim", [(19, 42, 42, 128), (300, 6, 1, 128), (5, 4, 4, 64),
+                                                       (2500, 5, 3, 64), (1, 1, 0, 128)])
+def test_norm_gradients_without_eps(K, tokens, heads, kv_heads, dim, dtype):  # noqa: F811
+    """Head counts that leave a batch of loads part empty: the empty places have no norm at eps = 0."""
+    torch.manual_seed(1)
+    q, k, qw, kw, dq, dk = norm_inputs(tokens, heads, kv_heads, dim, dtype)
+    check_norm_gradients(K, q, k, qw, kw, rope_of(tokens, dim, 3, True, "cuda"), dq, dk, 0.0)
