@@ -4,7 +4,7 @@
 //   n    = x * r,  r = 1 / sqrt(mean_d x^2 + eps)                 (normalising form)
 //   y    = R(a) (n * w)       (x0, x1) -> (x0 cos a - x1 sin a, x0 sin a + x1 cos a)
 // and backward, with g = R(-a) dy and gw = g * w:
-//   dx   = r * gw - x * r^3 * mean_d(gw * x),   dw = sum over tokens and heads of g * n
+//   dx   = r * (gw - n * mean_d(gw * n)),   dw = sum over tokens and heads of g * n
 //
 // Every element is read once and written once, so DRAM bandwidth is the bound.
 // A warp owns one token (or, in a call of few tokens, a run of its heads): its
@@ -344,11 +344,12 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
       // A place past h1 holds zeros and weighs nothing: without eps the r of its row would be infinite.
       const int at = h + u * kGroups + g;
       const float r = at < h1 ? rsqrtf(ss * (1.f / D) + p.eps) : 0.f;
-      const Four r4 = all4(r), back = all4(-r * r * r * (gx * (1.f / D)));
-      acc[0] = fma4(mul4(ga, r4), a, acc[0]);
-      acc[1] = fma4(mul4(gb, r4), b, acc[1]);
-      ya = fma4(a, back, mul4(gwa, r4));
-      yb = fma4(b, back, mul4(gwb, r4));
+      // dx = r (gw - n mean(gw n)) with n = r x.  Not x r^3 mean(gw x): at an rms of 1e15 r^3 has left fp32.
+      const Four r4 = all4(r), na = mul4(a, r4), nb = mul4(b, r4), back = all4(-(gx * r) * (1.f / D));
+      acc[0] = fma4(ga, na, acc[0]);
+      acc[1] = fma4(gb, nb, acc[1]);
+      ya = mul4(fma4(na, back, gwa), r4);
+      yb = mul4(fma4(nb, back, gwb), r4);
       if (at < h1) store_pairs<D, INTER>(dx + at * dx_head, l, ya, yb);
     }
   }

@@ -55,3 +55,23 @@ def test_norm_gradients_without_eps(K, tokens, heads, kv_heads, dim, dtype):  # 
     torch.manual_seed(1)
     q, k, qw, kw, dq, dk = norm_inputs(tokens, heads, kv_heads, dim, dtype)
     check_norm_gradients(K, q, k, qw, kw, rope_of(tokens, dim, 3, True, "cuda"), dq, dk, 0.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size,eps", [(1e15, 1e-6), (1e17, 0.0), (1e-14, 1e-30), (1e-16, 0.0)])
+def test_norm_gradients_of_large_and_small_rows(K, size, eps, dtype):  # noqa: F811
+    """1 / rms and its square are fp32 numbers where its cube is not."""
+    torch.manual_seed(2)
+    q, k, qw, kw, dq, dk = norm_inputs(50, 4, 3, 128, dtype, size)
+    check_norm_gradients(K, q, k, qw, kw, rope_of(50, 128, 3, False, "cuda"), dq, dk, eps)
+
+
+@gpu
+@pytest.mark.parametrize("eps", [1e-6, 1e-30])
+def test_norm_gradients_of_zero_rows(K, eps):  # noqa: F811
+    """A row of zeros has no direction: its gradient is w g / sqrt(eps), its part of the weights' is zero."""
+    torch.manual_seed(3)
+    q, k, qw, kw, dq, dk = norm_inputs(9, 3, 2, 64, torch.float32)
+    q[4], k[:, 1] = 0.0, 0.0
+    check_norm_gradients(K, q, k, qw, kw, None, dq, dk, eps)
