@@ -13,6 +13,7 @@
 #include <queue>
 
 #include "../common/launch.h"
+#include "../common/layout.h"
 #include "packed.h"
 #include "packed_api.h"
 
@@ -284,16 +285,6 @@ CUtensorMap query_map(const at::Tensor& t, int group, int bt) {
   const cuuint64_t strides[3] = {stride_bytes(t, 1), stride_bytes(t, 1) * group, stride_bytes(t, 0)};
   const cuuint32_t box[4] = {64u, static_cast<cuuint32_t>(group), 1u, static_cast<cuuint32_t>(bt)};
   return encode(t, 4, dims, strides, box);
-}
-
-// `t` itself if TMA and the kernels can read its layout (unit stride within a
-// head, every head on a 16-byte boundary, no zero stride), else a contiguous copy.
-at::Tensor fit(const at::Tensor& t) {
-  if (!t.is_cuda() || t.dim() != 3 || t.numel() == 0 || t.scalar_type() != at::kBFloat16) return t;
-  const bool fits = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
-                    (t.size(0) == 1 || (t.stride(0) > 0 && t.stride(0) % 8 == 0)) &&
-                    (t.size(1) == 1 || (t.stride(1) > 0 && t.stride(1) % 8 == 0));
-  return fits ? t : t.contiguous();
 }
 
 at::Tensor empty_cuda(at::IntArrayRef sizes, c10::ScalarType type, const at::Tensor& like) {

@@ -31,6 +31,7 @@
 #include <mutex>
 
 #include "../common/launch.h"
+#include "../common/layout.h"
 #include "../common/ptx.cuh"
 #include "qk_rope.h"
 
@@ -436,17 +437,6 @@ void check_heads(const at::Tensor& t, const char* what, const at::Tensor& q) {
                                  (t.size(1) == 1 || t.stride(1) % unit == 0) &&
                                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
               what, " must have unit stride within a head and heads on 16-byte boundaries");
-}
-
-// `t` itself if the kernels can read its layout (unit stride within a head,
-// every head on a 16-byte boundary, no zero stride), else a contiguous copy.
-at::Tensor fit(const at::Tensor& t) {
-  if (!t.is_cuda() || t.dim() != 3 || t.numel() == 0) return t;
-  const int64_t unit = 16 / t.element_size();
-  const bool fits = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
-                    (t.size(0) == 1 || (t.stride(0) > 0 && t.stride(0) % unit == 0)) &&
-                    (t.size(1) == 1 || (t.stride(1) > 0 && t.stride(1) % unit == 0));
-  return fits ? t : t.contiguous();
 }
 
 at::Tensor empty_cuda(at::IntArrayRef sizes, c10::ScalarType type, const at::Tensor& like) {

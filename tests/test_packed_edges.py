@@ -75,3 +75,40 @@ def test_norm_gradients_of_zero_rows(K, eps):  # noqa: F811
     q, k, qw, kw, dq, dk = norm_inputs(9, 3, 2, 64, torch.float32)
     q[4], k[:, 1] = 0.0, 0.0
     check_norm_gradients(K, q, k, qw, kw, None, dq, dk, eps)
+
+
+# ---------------------------------------------------------------- layouts
+def shifted(t, by=1):
+    """The same values in contiguous memory that starts `by` elements past a 16-byte boundary."""
+    flat = torch.empty(t.numel() + by, dtype=t.dtype, device=t.device)
+    return flat[by:].view(t.shape).copy_(t)
+
+
+@gpu
+@pytest.mark.parametrize("q_lens,heads,kv_heads", [([70, 33], 4, 2), ([1], 1, 1)])
+def test_attention_of_contiguous_tensors_off_a_boundary(K, q_lens, heads, kv_heads):  # noqa: F811
+    torch.manual_seed(4)
+    plan = K.packed_plan(q_lens, heads=heads, kv_heads=kv_heads, head_dim=64, causal=True)
+    n = plan.q_tokens
+    q, k, v, do = bf(n, heads, 64), bf(n, kv_heads, 64), bf(n, kv_heads, 64), bf(n, heads, 64)
+    o, lse = K.attention_packed_fwd(q, k, v, plan)
+    want = (o, lse) + K.attention_packed_bwd(q, k, v, o, lse, do, plan)
+    qs, ks, vs, os_, ds = (shifted(t) for t in (q, k, v, o, do))
+    assert all(t.is_contiguous() and t.data_ptr() % 16 for t in (qs, ks, vs, os_, ds))
+    got = K.attention_packed_fwd(qs, ks, vs, plan) + K.attention_packed_bwd(qs, ks, vs, os_, lse, ds, plan)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    K.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,heads", [(33, 3), (1, 1)])
+def test_rotation_and_norms_of_contiguous_tensors_off_a_boundary(K, tokens, heads, dtype):  # noqa: F811
+    torch.manual_seed(5)
+    rope = rope_of(tokens, 64, 3, True, "cuda")
+    q, k, qw, kw, dq, dk = norm_inputs(tokens, heads, heads, 64, dtype)
+    qs, ks, dqs, dks = (shifted(t) for t in (q, k, dq, dk))
+    want = K.rope_axes(q, k, rope) + K.qk_norm_rope(q, k, qw, kw, rope) + K.qk_norm_rope_bwd(q, k, qw, kw, rope, dq, dk)
+    got = K.rope_axes(qs, ks, rope) + K.qk_norm_rope(qs, ks, qw, kw, rope) + \
+        K.qk_norm_rope_bwd(qs, ks, qw, kw, rope, dqs, dks)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
