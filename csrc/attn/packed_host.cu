@@ -527,6 +527,7 @@ std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q_in, const at::T
   check_rows(grads[0], "dq", tq, hq, d, q.device());
   check_rows(grads[1], "dk", tk, hk, d, q.device());
   check_rows(grads[2], "dv", tk, hk, d, q.device());
+  if (!out.empty()) check_apart(out, {q, k, v, o, dout, lse});
   if (tq == 0 || tk == 0) {
     for (auto& g : grads) g.zero_();
     return grads;

@@ -605,9 +605,7 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
     check_heads(dq, "out dq", q);
     check_heads(dk, "out dk", q);
     TORCH_CHECK(dq.size(1) == q.size(1) && dk.size(1) == k.size(1), "out must have the heads of q and k");
-    for (const auto& t : out)
-      TORCH_CHECK((t.size(0) <= 1 || t.stride(0) > 0) && (t.size(1) <= 1 || t.stride(1) > 0),
-                  "out must not overlap itself");
+    check_apart(out, {q, k, dq_out, dk_out, q_weight, k_weight});
   }
   p.oq_tok = dq.stride(0), p.oq_head = dq.stride(1), p.ok_tok = dk.stride(0), p.ok_head = dk.stride(1);
   const int heads = p.Hq + p.Hk, D = static_cast<int>(q.size(2));

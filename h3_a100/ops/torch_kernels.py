@@ -341,10 +341,9 @@ class TorchKernels:
         scale = plan.head_dim ** -0.5 if scale is None else scale
         group = plan.heads // plan.kv_heads
         dtype = torch.promote_types(q.dtype, torch.float32)
-        grads = out if out is not None else tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device)
-                                                  for x in (q, k, v))
-        for g in grads:
-            g.zero_()
+        if out is not None and len(out) != 3:
+            raise ValueError("out must hold dq, dk and dv")
+        grads = tuple(torch.zeros(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
         for rq, rk, hidden in self._packed_sequences(plan, q.device):
             if rq.start == rq.stop or rk.start == rk.stop:
                 continue
@@ -363,7 +362,7 @@ class TorchKernels:
             grads[0][rq] = (ds @ ks).transpose(0, 1).to(grads[0].dtype)
             grads[1][rk] = per_key_head(ds.transpose(1, 2) @ qs).to(grads[1].dtype)
             grads[2][rk] = per_key_head(p.transpose(1, 2) @ dos).to(grads[2].dtype)
-        return tuple(grads)
+        return grads if out is None else tuple(o.copy_(g) for o, g in zip(out, grads))
 
     # ---------------- small projections ----------------
     def adaln_project(self, temb, w, b):

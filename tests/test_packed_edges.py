@@ -2,11 +2,16 @@
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 
+from h3_a100.ops import TorchKernels
 from test_packed_ops import K, U, bf, norm_turned, rope_of, turned  # noqa: F401  (K is a fixture)
 
+_C = pytest.importorskip("h3_a100._C")
+R = TorchKernels()
 gpu = pytest.mark.gpu
 
 
@@ -112,3 +117,90 @@ def test_rotation_and_norms_of_contiguous_tensors_off_a_boundary(K, tokens, head
     got = K.rope_axes(qs, ks, rope) + K.qk_norm_rope(qs, ks, qw, kw, rope) + \
         K.qk_norm_rope_bwd(qs, ks, qw, kw, rope, dqs, dks)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------- outputs in memory of the caller's
+def _bytes(t):
+    """Addresses of the elements of a view, one entry per place in its index space."""
+    at = torch.tensor(t.storage_offset())
+    for n, s in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    return at.reshape(-1)
+
+
+def _apart(out, ins=()):
+    try:
+        _C.check_apart(list(out), list(ins))
+    except RuntimeError as e:
+        assert "overlap" in str(e) or "over an input" in str(e)
+        return False
+    return True
+
+
+def test_overlaps_are_what_sets_of_addresses_say():
+    rng, flat, seen = random.Random(3), torch.zeros(4000), [0, 0, 0, 0]
+    for _ in range(4000):
+        views = []
+        fused = rng.random() < 0.5
+        row = rng.choice([16, 24, 40, 48])
+        for _ in range(2):
+            t, h, d = rng.randint(1, 6), rng.randint(1, 4), rng.choice([1, 2, 4, 8])
+            strides = (row, rng.choice([d, 8, 12, 16])) if fused else (rng.randint(0, 40), rng.randint(0, 40))
+            strides = strides if rng.random() < 0.7 else strides[::-1]
+            views.append(flat.as_strided((t, h, d), (*strides, 1), rng.randint(0, 120)))
+        a, b = (_bytes(v) for v in views)
+        folded, shared = a.unique().numel() < a.numel(), bool(set(a.tolist()) & set(b.tolist()))
+        assert _apart(views[:1]) == (not folded)
+        if not folded:
+            assert _apart(views[:1], views[1:]) == (not shared)
+            seen[int(shared)] += 1
+    assert min(seen[:2]) > 300
+
+
+def test_layouts_of_models_are_apart():
+    fused = torch.zeros(50, 8 * 64)
+    q, k, v = fused[:, :256].view(50, 4, 64), fused[:, 256:384].view(50, 2, 64), fused[:, 384:].view(50, 2, 64)
+    assert _apart([q, k, v]) and not _apart([q, k, k]) and not _apart([q, k], [fused])
+    assert not _apart([fused[:, 32:288].view(50, 4, 64)], [q])
+    turn = torch.zeros(50, 4, 3, 64)      # heads of q, k and v in turn
+    assert _apart(turn.unbind(2)) and _apart([turn[:, :1, 0], turn[:, :, 1]], [turn[:, 2:3, 0]])
+    first = torch.zeros(3, 4, 50, 64).transpose(1, 2)
+    assert _apart(first.unbind(0)) and _apart([first[0, :, :2], first[0, :, 2:]])
+    assert not _apart([first[0], first[0, 9:]])
+    assert _apart([torch.zeros(0, 4, 64), torch.zeros(0, 4, 64)], [q])
+    assert not _apart([torch.zeros(1, 4, 64).expand(50, -1, -1)])
+
+
+def test_torch_gradients_into_inputs():
+    """The PyTorch set writes after it has read."""
+    torch.manual_seed(8)
+    plan = R.packed_plan([5, 4], heads=2, kv_heads=2, head_dim=8, causal=True)
+    q, k, v, do = (torch.randn(9, 2, 8, dtype=torch.float64) for _ in range(4))
+    o, lse = R.attention_packed_fwd(q, k, v, plan)
+    want = R.attention_packed_bwd(q, k, v, o, lse, do, plan)
+    got = R.attention_packed_bwd(q, k, v, o, lse, do, plan, out=(q, k, v))
+    assert all(a is b for a, b in zip(got, (q, k, v))) and all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(ValueError, match="dq, dk and dv"):
+        R.attention_packed_bwd(q, k, v, o, lse, do, plan, out=(q, k))
+
+
+@gpu
+def test_gradients_over_inputs_or_each_other_are_refused(K):  # noqa: F811
+    plan = K.packed_plan([40, 9], heads=4, kv_heads=2, head_dim=64, causal=True)
+    q, k, v, do = bf(49, 4, 64), bf(49, 2, 64), bf(49, 2, 64), bf(49, 4, 64)
+    o, lse = K.attention_packed_fwd(q, k, v, plan)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    fused = bf(49, 8 * 64)
+    for out, message in (((dq, dk, dk), "each other"), ((q, dk, dv), "over an input"), ((do, dk, dv), "over an input"),
+                         ((o, dk, dv), "over an input"), ((dq, k, dv), "over an input"), ((dq, dk, v), "over an input"),
+                         ((fused[:, :256].view(49, 4, 64), fused[:, 192:320].view(49, 2, 64), dv), "each other"),
+                         ((dq, bf(50 * 64).as_strided((49, 2, 64), (64, 64, 1)), dv), "overlap itself")):
+        with pytest.raises(RuntimeError, match=message):
+            K.attention_packed_bwd(q, k, v, o, lse, do, plan, out=out)
+    rope, w = rope_of(49, 64, 3, True, "cuda"), bf(64)
+    dk_in = bf(49, 2, 64)
+    for out, message in (((q, dk), "over an input"), ((dq, dk_in), "over an input"), ((do, dk), "over an input"),
+                         ((fused[:, :256].view(49, 4, 64), fused[:, 192:320].view(49, 2, 64)), "each other"),
+                         ((dq, bf(50 * 64).as_strided((49, 2, 64), (64, 64, 1))), "overlap itself")):
+        with pytest.raises(RuntimeError, match=message):
+            K.qk_norm_rope_bwd(q, k, w, w, rope, do, dk_in, out=out)
