@@ -2,6 +2,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -313,6 +314,15 @@ void check_plan(const at::Tensor& q, const at::Tensor& blob, const std::vector<i
               "not a packed schedule");
 }
 
+// The stream that the kernels run on.  The plan's memory is the plan's, not the
+// caller's to look after: it must not be given out again while they read it,
+// also where the plan was made on another stream and is dropped after the call.
+cudaStream_t stream_for(const at::Tensor& q, const at::Tensor& blob) {
+  const c10::cuda::CUDAStream stream = at::cuda::getCurrentCUDAStream(q.get_device());
+  c10::cuda::CUDACachingAllocator::recordStream(blob.storage().data_ptr(), stream);
+  return stream.stream();
+}
+
 void check_scale(double scale) {
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite, got ", scale);
 }
@@ -488,7 +498,7 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q_in, const at::T
     p.part_rows = static_cast<int>(meta[kPartRows]);
     p.part_extent = rows * head_dim;
   }
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
+  const cudaStream_t stream = stream_for(q, blob);
   launch_packed_fwd(head_dim, meta[kFew] != 0, static_cast<int>(meta[kFwdBlocks]), query_map(q, p.G, p.bt),
                     key_map(k), key_map(v), p, stream);
   after_launch();
@@ -558,7 +568,7 @@ std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q_in, const at::T
   p.dq_extent = extent(grads[0]), p.dk_extent = extent(grads[1]), p.dv_extent = extent(grads[2]);
   p.status.word = status.data_ptr<int>();
   p.status.limit_ns = static_cast<uint64_t>(limit_ns);
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream(q.get_device()).stream();
+  const cudaStream_t stream = stream_for(q, blob);
   const CUtensorMap mq = query_map(q, p.G, p.bt), mdo = query_map(dout, p.G, p.bt), mk = key_map(k), mv = key_map(v);
   launch_packed_delta(head_dim, p, stream);
   after_launch();

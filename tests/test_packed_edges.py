@@ -204,3 +204,29 @@ def test_gradients_over_inputs_or_each_other_are_refused(K):  # noqa: F811
                          ((dq, bf(50 * 64).as_strided((49, 2, 64), (64, 64, 1))), "overlap itself")):
         with pytest.raises(RuntimeError, match=message):
             K.qk_norm_rope_bwd(q, k, w, w, rope, do, dk_in, out=out)
+
+
+@gpu
+def test_a_plan_dropped_while_another_stream_reads_it(K):  # noqa: F811
+    """Its memory is not given to the next tensor of its own stream before the kernels are done."""
+    torch.manual_seed(9)
+    q_lens = [300, 41, 7]
+    plan = K.packed_plan(q_lens, heads=4, kv_heads=2, head_dim=64, causal=True)
+    q, k, v, do = bf(348, 4, 64), bf(348, 2, 64), bf(348, 2, 64), bf(348, 4, 64)
+    want = K.attention_packed_fwd(q, k, v, plan)
+    want += K.attention_packed_bwd(q, k, v, *want, do, plan)
+    at, size = plan.blob.data_ptr(), plan.blob.numel()
+    side, busy = torch.cuda.Stream(), torch.cuda.Event()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)      # about a tenth of a second
+        got = K.attention_packed_fwd(q, k, v, plan)
+        got += K.attention_packed_bwd(q, k, v, *got, do, plan)
+        busy.record()
+    del plan
+    other = [torch.full((size,), -1, dtype=torch.int32, device="cuda") for _ in range(4)]
+    assert not busy.query(), "the side stream was not behind"
+    assert all(t.data_ptr() != at for t in other)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    K.check_status()
