@@ -323,8 +323,11 @@ cudaStream_t stream_for(const at::Tensor& q, const at::Tensor& blob) {
   return stream.stream();
 }
 
+// The kernels hold the scale and its product with log2(e) in fp32.
+constexpr double kLog2e = 1.4426950408889634;
 void check_scale(double scale) {
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite, got ", scale);
+  const float low = static_cast<float>(scale), high = static_cast<float>(scale * kLog2e);
+  TORCH_CHECK(low > 0 && std::isfinite(high), "scale must be positive and finite in fp32, got ", scale);
 }
 
 void check_status_word(const at::Tensor& status, const at::Tensor& q) {
@@ -483,7 +486,7 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q_in, const at::T
   p.bt = 128 / p.G;
   p.Hq = static_cast<int>(meta[kHq]);
   p.Tq = meta[kTq];
-  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.scale_log2 = static_cast<float>(scale * kLog2e);
   p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
   p.lse = lse.data_ptr<float>();
   p.o_extent = extent(o);
@@ -552,7 +555,7 @@ std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q_in, const at::T
   p.Hq = static_cast<int>(hq), p.Hk = static_cast<int>(hk);
   p.Tq = tq, p.Tk = tk;
   p.scale = static_cast<float>(scale);
-  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.scale_log2 = static_cast<float>(scale * kLog2e);
   p.o = reinterpret_cast<const __nv_bfloat16*>(o.data_ptr());
   p.dout = reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr());
   p.o_tok = o.stride(0), p.o_head = o.stride(1), p.do_tok = dout.stride(0), p.do_head = dout.stride(1);

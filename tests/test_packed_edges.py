@@ -230,3 +230,21 @@ def test_a_plan_dropped_while_another_stream_reads_it(K):  # noqa: F811
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     K.check_status()
+
+
+# ---------------------------------------------------------------- scales
+@gpu
+def test_attention_scales_at_the_ends_of_fp32(K):  # noqa: F811
+    """The kernels hold scale and scale * log2(e) in fp32: what is 0 or infinite there is refused."""
+    torch.manual_seed(6)
+    plan = K.packed_plan([40, 9], heads=2, kv_heads=1, head_dim=64, causal=True)
+    q, k, v = bf(49, 2, 64), bf(49, 1, 64), bf(49, 1, 64)
+    o, lse = K.attention_packed_fwd(q, k, v, plan, scale=1e-30)
+    # scores of 1e-28: every visible key weighs the same
+    seen = torch.cat([torch.arange(1, n + 1, device="cuda") for n in (40, 9)])
+    assert ((lse.double() - seen.double().log()).abs() <= 2.0 ** -19).all()
+    for scale in (1e-60, 1e39, 3e38):
+        with pytest.raises(RuntimeError, match="scale"):
+            K.attention_packed_fwd(q, k, v, plan, scale=scale)
+        with pytest.raises(RuntimeError, match="scale"):
+            K.attention_packed_bwd(q, k, v, o, lse, q, plan, scale=scale)
