@@ -443,6 +443,18 @@ at::Tensor empty_cuda(at::IntArrayRef sizes, c10::ScalarType type, const at::Ten
   return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
+// Positions, frequencies and weights are read with unit stride: `t`, or a copy kept in `copy`.
+using OptionalTensor = c10::optional<at::Tensor>;
+bool is_dense(const at::Tensor& t) { return t.dim() == 0 || t.stride(t.dim() - 1) == 1; }
+const OptionalTensor& dense(const OptionalTensor& t, OptionalTensor& copy) {
+  if (!t.has_value() || is_dense(*t)) return t;
+  copy = t->contiguous();
+  return copy;
+}
+const at::Tensor& dense(const at::Tensor& t, at::Tensor& copy) {
+  return is_dense(t) ? t : copy = t.contiguous();
+}
+
 RopeParams make_params(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& positions,
                        const c10::optional<at::Tensor>& freqs, const std::vector<int64_t>& pairs, bool inverse,
                        double eps) {
@@ -541,10 +553,14 @@ void dispatch(const at::Tensor& q, bool interleaved, F&& f) {
 }  // namespace
 
 std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q_in, const c10::optional<at::Tensor>& k_in,
-                                    const c10::optional<at::Tensor>& q_weight,
-                                    const c10::optional<at::Tensor>& k_weight,
-                                    const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& freqs,
-                                    const std::vector<int64_t>& pairs, bool interleaved, bool inverse, double eps) {
+                                    const c10::optional<at::Tensor>& q_weight_in,
+                                    const c10::optional<at::Tensor>& k_weight_in,
+                                    const c10::optional<at::Tensor>& positions_in,
+                                    const c10::optional<at::Tensor>& freqs_in, const std::vector<int64_t>& pairs,
+                                    bool interleaved, bool inverse, double eps) {
+  OptionalTensor copies[4];
+  const OptionalTensor &q_weight = dense(q_weight_in, copies[0]), &k_weight = dense(k_weight_in, copies[1]);
+  const OptionalTensor &positions = dense(positions_in, copies[2]), &freqs = dense(freqs_in, copies[3]);
   const at::Tensor q = fit(q_in);
   const at::Tensor k = k_in.has_value() ? fit(*k_in) : q.narrow(1, 0, 0);
   RopeParams p = make_params(q, k, positions, freqs, pairs, inverse, eps);
@@ -582,11 +598,16 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q_in, const c10::optional<
   return {q_out, k_out};
 }
 
-std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& q_weight,
-                                         const at::Tensor& k_weight, const c10::optional<at::Tensor>& positions,
-                                         const c10::optional<at::Tensor>& freqs, const std::vector<int64_t>& pairs,
+std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tensor& k_in,
+                                         const at::Tensor& q_weight_in, const at::Tensor& k_weight_in,
+                                         const c10::optional<at::Tensor>& positions_in,
+                                         const c10::optional<at::Tensor>& freqs_in, const std::vector<int64_t>& pairs,
                                          bool interleaved, const at::Tensor& dq_in, const at::Tensor& dk_in,
                                          double eps, const std::vector<at::Tensor>& out) {
+  at::Tensor weight_copies[2];
+  OptionalTensor copies[2];
+  const at::Tensor &q_weight = dense(q_weight_in, weight_copies[0]), &k_weight = dense(k_weight_in, weight_copies[1]);
+  const OptionalTensor &positions = dense(positions_in, copies[0]), &freqs = dense(freqs_in, copies[1]);
   const at::Tensor q = fit(q_in), k = fit(k_in), dq_out = fit(dq_in), dk_out = fit(dk_in);
   RopeParams p = make_params(q, k, positions, freqs, pairs, false, eps);
   bool kb = false;

@@ -7,7 +7,7 @@ import random
 import pytest
 import torch
 
-from h3_a100.ops import TorchKernels
+from h3_a100.ops import AxisRope, TorchKernels
 from test_packed_ops import K, U, bf, norm_turned, rope_of, turned  # noqa: F401  (K is a fixture)
 
 _C = pytest.importorskip("h3_a100._C")
@@ -248,3 +248,18 @@ def test_attention_scales_at_the_ends_of_fp32(K):  # noqa: F811
             K.attention_packed_fwd(q, k, v, plan, scale=scale)
         with pytest.raises(RuntimeError, match="scale"):
             K.attention_packed_bwd(q, k, v, o, lse, q, plan, scale=scale)
+
+
+@gpu
+def test_strided_positions_frequencies_and_weights(K):  # noqa: F811
+    torch.manual_seed(7)
+    rope = rope_of(21, 64, 3, True, "cuda")
+    strided = AxisRope(rope.positions.t().contiguous().t(), rope.freqs.repeat_interleave(2)[::2], rope.pairs)
+    assert strided.positions.stride() == (1, 21) and strided.freqs.stride() == (2,)
+    q, k, qw, kw, dq, dk = norm_inputs(21, 3, 2, 64, torch.bfloat16)
+    w2, w3 = torch.stack([qw, kw], 1).unbind(1)
+    assert not w2.is_contiguous()
+    want = K.rope_axes(q, k, rope) + K.qk_norm_rope(q, k, qw, kw, rope) + K.qk_norm_rope_bwd(q, k, qw, kw, rope, dq, dk)
+    got = K.rope_axes(q, k, strided) + K.qk_norm_rope(q, k, w2, w3, strided) + \
+        K.qk_norm_rope_bwd(q, k, w2, w3, strided, dq, dk)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
