@@ -204,8 +204,11 @@ class NativeKernels:
             return None, None, [], True
         return rope.positions, rope.freqs, rope.pairs, rope.interleaved
 
-    def rope_axes(self, q, k, rope: AxisRope, inverse: bool = False):
-        """Rotate every head of ``q`` and ``k`` (``k`` may be None); ``inverse`` turns gradients back."""
+    def rope_axes(self, q, k, rope: AxisRope | None, inverse: bool = False):
+        """Rotate every head of ``q`` and ``k`` (``k`` may be None); ``inverse`` turns gradients back.
+
+        Without a ``rope`` nothing turns and the results are copies.
+        """
         pos, freqs, pairs, inter = self._rope_args(rope)
         both = self.C.qk_rope_fwd(q, k, None, None, pos, freqs, pairs, inter, bool(inverse), 0.0)
         return both[0], None if k is None else both[1]

@@ -246,11 +246,14 @@ class TorchKernels:
         y = a * cos - b * sin, a * sin + b * cos
         return torch.stack(y, -1).flatten(-2) if interleaved else torch.cat(y, -1)
 
-    def rope_axes(self, q, k, rope: AxisRope, inverse: bool = False):
-        """Rotate every head of ``q`` and ``k`` (``k`` may be None); ``inverse`` turns gradients back."""
+    def rope_axes(self, q, k, rope: AxisRope | None, inverse: bool = False):
+        """Rotate every head of ``q`` and ``k`` (``k`` may be None); ``inverse`` turns gradients back.
+
+        Without a ``rope`` nothing turns and the results are copies.
+        """
         cos, sin = self._axis_tables(rope, q.shape[-1], q)
-        sin = -sin if inverse else sin
-        return tuple(None if x is None else self._turn(x.to(cos.dtype), cos, sin, rope.interleaved).to(x.dtype)
+        sin, interleaved = -sin if inverse else sin, rope is None or rope.interleaved
+        return tuple(None if x is None else self._turn(x.to(cos.dtype), cos, sin, interleaved).to(x.dtype)
                      for x in (q, k))
 
     def qk_norm_rope(self, q, k, q_weight, k_weight, rope: AxisRope | None = None, eps=1e-6):

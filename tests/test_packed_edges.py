@@ -263,3 +263,16 @@ def test_strided_positions_frequencies_and_weights(K):  # noqa: F811
     got = K.rope_axes(q, k, strided) + K.qk_norm_rope(q, k, w2, w3, strided) + \
         K.qk_norm_rope_bwd(q, k, w2, w3, strided, dq, dk)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_rotation_is_a_copy():
+    q, k = torch.randn(7, 3, 8).bfloat16(), torch.randn(7, 2, 8).bfloat16()
+    for got, x in zip(R.rope_axes(q, k, None) + R.rope_axes(q, k, None, inverse=True), (q, k, q, k)):
+        assert torch.equal(got, x) and got.data_ptr() != x.data_ptr()
+
+
+@gpu
+def test_no_rotation_is_a_copy_on_the_gpu(K):  # noqa: F811
+    q, k = bf(7, 3, 64), bf(7, 2, 64)
+    for got, x in zip(K.rope_axes(q, k, None) + K.rope_axes(q, k, None, inverse=True), (q, k, q, k)):
+        assert torch.equal(got, x) and got.data_ptr() != x.data_ptr()
