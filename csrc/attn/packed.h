@@ -46,7 +46,7 @@ struct PackedFwdParams {
   float* part_o;           // [slots, rows, D] normalised parts
   float* part_lse;         // [slots, rows] log2
   int part_rows;
-  long o_extent, lse_extent, part_extent;   // allocation extents (bounds-checked build)
+  long o_extent, lse_extent, part_extent, part_lse_extent;   // allocation extents (bounds-checked build)
   KernelStatus status;
 };
 
@@ -64,7 +64,7 @@ struct PackedBwdParams {
   float* delta;            // [Hq, Tq]
   __nv_bfloat16 *dq, *dk, *dv;
   long dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
-  long dq_extent, dk_extent, dv_extent;
+  long row_extent, dq_extent, dk_extent, dv_extent;   // allocation extents (lse2 and delta: each)
   KernelStatus status;
 };
 

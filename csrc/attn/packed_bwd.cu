@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(PackedBwdParams p) {
       const int kh = h / p.G, g = h - kh * p.G;
       const long row = (kh * p.Tq + t) * p.G + g;
       const float lse = p.lse[h * p.Tq + t];
+      if (!H3_IN_BOUNDS(row, row, p.row_extent, p.status)) continue;
       p.delta[row] = s;
       p.lse2[row] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
     }
@@ -432,8 +433,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const float exact = exchange[row] + exchange[128 + row];
         neg_delta = pack2(-exact, -exact);
-        if (live && wg == 0)      // dk / dv reads it
-          p.delta[(it.head * p.Tq + it.q0 + row / p.G) * p.G + row % p.G] = exact;
+        const long at = (it.head * p.Tq + it.q0 + row / p.G) * p.G + row % p.G;
+        if (live && wg == 0 && H3_IN_BOUNDS(at, at, p.row_extent, p.status)) p.delta[at] = exact;   // dk / dv reads it
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {

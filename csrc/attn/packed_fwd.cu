@@ -454,7 +454,7 @@ __device__ __forceinline__ void softmax_warps(const PackedFwdParams& p, const Ba
     const long lse_off = static_cast<long>(head) * p.Tq + q;
     if (!both || t == 0) {
       if (live && part) {
-        p.part_lse[part_row] = lse2;
+        if (H3_IN_BOUNDS(part_row, part_row, p.part_lse_extent, p.status)) p.part_lse[part_row] = lse2;
       } else if (live && H3_IN_BOUNDS(lse_off, lse_off, p.lse_extent, p.status)) {
         p.lse[lse_off] = lse2 * 0.6931471805599453f;
       }

@@ -330,16 +330,6 @@ void check_scale(double scale) {
   TORCH_CHECK(low > 0 && std::isfinite(high), "scale must be positive and finite in fp32, got ", scale);
 }
 
-void check_status_word(const at::Tensor& status, const at::Tensor& q) {
-  TORCH_CHECK(status.device() == q.device() && status.scalar_type() == at::kInt && status.numel() >= 4,
-              "status must be int32[4] on q's device");
-}
-
-// Elements from the first one to the end of the storage (bounds-checked build).
-long extent(const at::Tensor& t) {
-  return static_cast<long>(t.storage().nbytes() / t.element_size()) - static_cast<long>(t.storage_offset());
-}
-
 // Sets the kernels' attributes once per device; the flags are F's own.
 template <const char* (*F)()>
 void configure_once() {
@@ -499,7 +489,8 @@ std::vector<at::Tensor> attention_packed_fwd(const at::Tensor& q_in, const at::T
     p.part_o = parts.data_ptr<float>();
     p.part_lse = p.part_o + rows * head_dim;
     p.part_rows = static_cast<int>(meta[kPartRows]);
-    p.part_extent = rows * head_dim;
+    p.part_extent = declared(rows * head_dim);
+    p.part_lse_extent = declared(rows);
   }
   const cudaStream_t stream = stream_for(q, blob);
   launch_packed_fwd(head_dim, meta[kFew] != 0, static_cast<int>(meta[kFwdBlocks]), query_map(q, p.G, p.bt),
@@ -568,6 +559,7 @@ std::vector<at::Tensor> attention_packed_bwd(const at::Tensor& q_in, const at::T
   p.dq_tok = grads[0].stride(0), p.dq_head = grads[0].stride(1);
   p.dk_tok = grads[1].stride(0), p.dk_head = grads[1].stride(1);
   p.dv_tok = grads[2].stride(0), p.dv_head = grads[2].stride(1);
+  p.row_extent = declared(hq * tq);
   p.dq_extent = extent(grads[0]), p.dk_extent = extent(grads[1]), p.dv_extent = extent(grads[2]);
   p.status.word = status.data_ptr<int>();
   p.status.limit_ns = static_cast<uint64_t>(limit_ns);

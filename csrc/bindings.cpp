@@ -27,6 +27,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_packed_bwd", &h3::attention_packed_bwd, "tcgen05 attention over packed sequences, backward");
   m.def("qk_rope_fwd", &h3::qk_rope_fwd, "multi-axis rotation of q and k, with their norms if weights are given");
   m.def("qk_norm_rope_bwd", &h3::qk_norm_rope_bwd, "gradients of the norm and rotation of q and k");
+  m.attr("bounds_checked") = h3::kBoundsChecked;
   m.def("check_apart", &h3::check_apart, "raises where an output tensor overlaps itself, another one or an input");
   m.def("p2p_all_gather", &h3::p2p_all_gather, "pull all-gather over peer memory");
   m.def("p2p_all_gather_ce", &h3::p2p_all_gather_ce, "all-gather over peer memory on the copy engines");

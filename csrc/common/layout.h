@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 #include <utility>
 #include <vector>
 
@@ -19,6 +20,29 @@ inline at::Tensor fit(const at::Tensor& t) {
                     (t.size(0) == 1 || (t.stride(0) > 0 && t.stride(0) % unit == 0)) &&
                     (t.size(1) == 1 || (t.stride(1) > 0 && t.stride(1) % unit == 0));
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Elements that a kernel may touch from a pointer on, which only the bounds-checked build asks for.
+// H3_BOUNDS_SHRINK=n, a test hook, declares each allocation n elements shorter.
+#ifdef H3_BOUNDS_CHECK
+constexpr bool kBoundsChecked = true;
+inline long declared(long elements) {
+  const char* shrink = std::getenv("H3_BOUNDS_SHRINK");
+  return elements - (shrink != nullptr ? std::atol(shrink) : 0);
+}
+// From the first element of `t` to the end of its storage.
+inline long extent(const at::Tensor& t) {
+  return declared(static_cast<long>(t.storage().nbytes() / t.element_size()) - static_cast<long>(t.storage_offset()));
+}
+#else
+constexpr bool kBoundsChecked = false;
+inline long declared(long) { return 0; }
+inline long extent(const at::Tensor&) { return 0; }
+#endif
+
+inline void check_status_word(const at::Tensor& status, const at::Tensor& q) {
+  TORCH_CHECK(status.device() == q.device() && status.scalar_type() == at::kInt && status.numel() >= 4,
+              "status must be int32[4] on q's device");
 }
 
 // The bytes of a tensor of up to three dimensions with unit stride in the last one: segments of `len` bytes in two

@@ -54,6 +54,10 @@ struct RopeParams {
   int end[kMaxAxes];            // pairs below end[a] rotate by the first axis a for which this holds
   float sign, eps;
   bool w_bf16;
+#ifdef H3_BOUNDS_CHECK      // only there: 40 bytes more of arguments cost a launch 0.3 us
+  long q_extent, k_extent, partial_extent;      // allocation extents
+  KernelStatus status;
+#endif
 };
 
 template <typename T>
@@ -240,11 +244,12 @@ __device__ __forceinline__ void weights(const void* w, bool bf16, int l, Four& f
   second4 = four(b[0], b[1], b[2], b[3]);
 }
 
-// Heads [h0, h1) of one token: x -> y (contiguous heads).
-template <typename T, int D, bool INTER, bool NORM>
-__device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head, T* __restrict__ y, int h0, int h1,
-                                              const void* w, const RopeParams& p, long t, bool& turned, Four& c,
+// Heads [h0, h1) of one token: x -> out + row (contiguous heads).
+template <typename T, int D, bool INTER, bool NORM, bool KEYS>
+__device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head, T* __restrict__ out, long row, int h0,
+                                              int h1, const void* w, const RopeParams& p, long t, bool& turned, Four& c,
                                               Four& s) {
+  T* const y = out + row;
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 4 : 2;
   const int g = lane_id() / kLanes, l = lane_id() % kLanes;
   Four wa, wb;
@@ -276,7 +281,8 @@ __device__ __forceinline__ void forward_heads(const T* __restrict__ x, long head
       }
       const Four ya = fma4(b, neg_s, mul4(a, c)), yb = fma4(b, c, mul4(a, s));
       const int at = h + u * kGroups + g;
-      if (at < h1) store_pairs<D, INTER>(y + at * D, l, ya, yb);
+      if (at < h1 && H3_IN_BOUNDS(row + at * D, row + at * D + D - 1, KEYS ? p.k_extent : p.q_extent, p.status))
+        store_pairs<D, INTER>(y + at * D, l, ya, yb);
     }
   }
 }
@@ -293,20 +299,19 @@ __global__ void __launch_bounds__(kThreads)
   Four c, s;
   bool turned = false;
   if (h0 < p.Hq)
-    forward_heads<T, D, INTER, NORM>(q + t * p.q_tok, p.q_head, q_out + t * p.Hq * D, h0, min(h1, p.Hq), qw, p, t,
-                                     turned, c, s);
+    forward_heads<T, D, INTER, NORM, false>(q + t * p.q_tok, p.q_head, q_out, t * p.Hq * D, h0, min(h1, p.Hq), qw, p, t,
+                                            turned, c, s);
   if (h1 > p.Hq)
-    forward_heads<T, D, INTER, NORM>(k + t * p.k_tok, p.k_head, k_out + t * p.Hk * D, max(h0 - p.Hq, 0), h1 - p.Hq, kw,
-                                     p, t, turned, c, s);
+    forward_heads<T, D, INTER, NORM, true>(k + t * p.k_tok, p.k_head, k_out, t * p.Hk * D, max(h0 - p.Hq, 0), h1 - p.Hq,
+                                           kw, p, t, turned, c, s);
 }
 
-// Heads [h0, h1) of one token: dy -> dx; adds to the lane's eight columns of the weight gradient.
-template <typename T, int D, bool INTER>
+// Heads [h0, h1) of one token: dy -> out + row; adds to the lane's eight columns of the weight gradient.
+template <typename T, int D, bool INTER, bool KEYS>
 __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long head, const T* __restrict__ dy,
-                                               long dy_head, T* __restrict__ dx, long dx_head, int h0, int h1,
-                                               const void* w,
-                                               const RopeParams& p, long t, bool& turned, Four& c,
-                                               Four& s, Four (&acc)[2]) {
+                                               long dy_head, T* __restrict__ out, long row, long dx_head, int h0,
+                                               int h1, const void* w, const RopeParams& p, long t, bool& turned,
+                                               Four& c, Four& s, Four (&acc)[2]) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kBatch = sizeof(T) == 2 ? 2 : 1;
   const int g = lane_id() / kLanes, l = lane_id() % kLanes;
   Four wa, wb;
@@ -351,7 +356,9 @@ __device__ __forceinline__ void backward_heads(const T* __restrict__ x, long hea
       acc[1] = fma4(gb, nb, acc[1]);
       ya = mul4(fma4(na, back, gwa), r4);
       yb = mul4(fma4(nb, back, gwb), r4);
-      if (at < h1) store_pairs<D, INTER>(dx + at * dx_head, l, ya, yb);
+      const long first = row + at * dx_head;
+      if (at < h1 && H3_IN_BOUNDS(first, first + D - 1, KEYS ? p.k_extent : p.q_extent, p.status))
+        store_pairs<D, INTER>(out + first, l, ya, yb);
     }
   }
 }
@@ -380,11 +387,11 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks)
     Four c, s;
     bool turned = false;
     if (h0 < p.Hq)
-      backward_heads<T, D, INTER>(q + t * p.q_tok, p.q_head, dyq + t * p.dq_tok, p.dq_head, dq + t * p.oq_tok,
-                                  p.oq_head, h0, min(h1, p.Hq), qw, p, t, turned, c, s, acc[0]);
+      backward_heads<T, D, INTER, false>(q + t * p.q_tok, p.q_head, dyq + t * p.dq_tok, p.dq_head, dq, t * p.oq_tok,
+                                         p.oq_head, h0, min(h1, p.Hq), qw, p, t, turned, c, s, acc[0]);
     if (h1 > p.Hq)
-      backward_heads<T, D, INTER>(k + t * p.k_tok, p.k_head, dyk + t * p.dk_tok, p.dk_head, dk + t * p.ok_tok,
-                                  p.ok_head, max(h0 - p.Hq, 0), h1 - p.Hq, kw, p, t, turned, c, s, acc[1]);
+      backward_heads<T, D, INTER, true>(k + t * p.k_tok, p.k_head, dyk + t * p.dk_tok, p.dk_head, dk, t * p.ok_tok,
+                                        p.ok_head, max(h0 - p.Hq, 0), h1 - p.Hq, kw, p, t, turned, c, s, acc[1]);
   }
   // Sum the lane groups in a fixed order: groups of a warp by shuffles, then the warps through shared memory.
   __shared__ float red[kBwdThreads / 32][2 * D];
@@ -405,7 +412,8 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks)
     float v = 0.f;
 #pragma unroll
     for (int wp = 0; wp < kBwdThreads / 32; ++wp) v += red[wp][i];
-    partial[static_cast<long>(blockIdx.x) * 2 * D + i] = v;
+    const long at = static_cast<long>(blockIdx.x) * 2 * D + i;
+    if (H3_IN_BOUNDS(at, at, p.partial_extent, p.status)) partial[at] = v;
   }
 }
 
@@ -498,6 +506,16 @@ RopeParams make_params(const at::Tensor& q, const at::Tensor& k, const c10::opti
   return p;
 }
 
+// What the bounds-checked build checks the stores against, and where it reports.
+void set_extents(RopeParams& p, const at::Tensor& q_out, const at::Tensor& k_out, const OptionalTensor& status) {
+#ifdef H3_BOUNDS_CHECK
+  TORCH_CHECK(status.has_value(), "the bounds-checked build needs the status word");
+  check_status_word(*status, q_out);
+  p.status.word = status->data_ptr<int>();
+  p.q_extent = extent(q_out), p.k_extent = extent(k_out);
+#endif
+}
+
 const void* check_weight(const at::Tensor& w, const at::Tensor& q, const char* what, bool& bf16) {
   TORCH_CHECK(w.device() == q.device() && w.is_contiguous() && w.numel() == q.size(2) && w.dim() == 1 &&
                   (w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16),
@@ -557,7 +575,8 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q_in, const c10::optional<
                                     const c10::optional<at::Tensor>& k_weight_in,
                                     const c10::optional<at::Tensor>& positions_in,
                                     const c10::optional<at::Tensor>& freqs_in, const std::vector<int64_t>& pairs,
-                                    bool interleaved, bool inverse, double eps) {
+                                    bool interleaved, bool inverse, double eps,
+                                    const OptionalTensor& status) {
   OptionalTensor copies[4];
   const OptionalTensor &q_weight = dense(q_weight_in, copies[0]), &k_weight = dense(k_weight_in, copies[1]);
   const OptionalTensor &positions = dense(positions_in, copies[2]), &freqs = dense(freqs_in, copies[3]);
@@ -575,6 +594,7 @@ std::vector<at::Tensor> qk_rope_fwd(const at::Tensor& q_in, const c10::optional<
   c10::cuda::CUDAGuard guard(q.get_device());
   auto q_out = empty_cuda(q.sizes(), q.scalar_type(), q);
   auto k_out = empty_cuda(k.sizes(), k.scalar_type(), k);
+  set_extents(p, q_out, k_out, status);
   const int heads = p.Hq + p.Hk, D = static_cast<int>(q.size(2));
   if (p.T == 0 || heads == 0) return {q_out, k_out};
   plan_runs(p, heads, D, static_cast<int>(q.element_size()));
@@ -603,7 +623,7 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
                                          const c10::optional<at::Tensor>& positions_in,
                                          const c10::optional<at::Tensor>& freqs_in, const std::vector<int64_t>& pairs,
                                          bool interleaved, const at::Tensor& dq_in, const at::Tensor& dk_in,
-                                         double eps, const std::vector<at::Tensor>& out) {
+                                         double eps, const OptionalTensor& status, const std::vector<at::Tensor>& out) {
   at::Tensor weight_copies[2];
   OptionalTensor copies[2];
   const at::Tensor &q_weight = dense(q_weight_in, weight_copies[0]), &k_weight = dense(k_weight_in, weight_copies[1]);
@@ -628,6 +648,7 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
     TORCH_CHECK(dq.size(1) == q.size(1) && dk.size(1) == k.size(1), "out must have the heads of q and k");
     check_apart(out, {q, k, dq_out, dk_out, q_weight, k_weight});
   }
+  set_extents(p, dq, dk, status);
   p.oq_tok = dq.stride(0), p.oq_head = dq.stride(1), p.ok_tok = dk.stride(0), p.ok_head = dk.stride(1);
   const int heads = p.Hq + p.Hk, D = static_cast<int>(q.size(2));
   if (p.T == 0 || heads == 0) {
@@ -645,6 +666,9 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& q_in, const at::Tenso
     const long blocks = (p.T * p.runs + kBwdThreads / 32 - 1) / (kBwdThreads / 32);
     const int grid = static_cast<int>(std::min<long>(blocks, resident_blocks(kernel, kBwdThreads)));
     auto partial = empty_cuda({grid, 2 * kD}, at::kFloat, q);
+#ifdef H3_BOUNDS_CHECK
+    p.partial_extent = extent(partial);
+#endif
     launch_overlapped(kernel, grid, kBwdThreads, 0, stream, reinterpret_cast<const T*>(q.data_ptr()),
                       reinterpret_cast<const T*>(k.data_ptr()), qw, kw, reinterpret_cast<const T*>(dq_out.data_ptr()),
                       reinterpret_cast<const T*>(dk_out.data_ptr()), reinterpret_cast<T*>(dq.data_ptr()),

@@ -59,6 +59,7 @@ class NativeKernels:
         self.device = device
         self.C = extension if extension is not None else _C
         self.status = torch.zeros(4, dtype=torch.int32, device=device)
+        self._reports = self.status if self.C.bounds_checked else None    # of kernels that wait for nothing
         self.limit_ns = int(wait_limit_s * 1e9)
         self.sms = _num_sms(device)
         self._ones = torch.ones(1, dtype=torch.float32, device=device)
@@ -210,13 +211,14 @@ class NativeKernels:
         Without a ``rope`` nothing turns and the results are copies.
         """
         pos, freqs, pairs, inter = self._rope_args(rope)
-        both = self.C.qk_rope_fwd(q, k, None, None, pos, freqs, pairs, inter, bool(inverse), 0.0)
+        both = self.C.qk_rope_fwd(q, k, None, None, pos, freqs, pairs, inter, bool(inverse), 0.0, self._reports)
         return both[0], None if k is None else both[1]
 
     def qk_norm_rope(self, q, k, q_weight, k_weight, rope: AxisRope | None = None, eps=1e-6):
         """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``), then the rotation."""
         pos, freqs, pairs, inter = self._rope_args(rope)
-        both = self.C.qk_rope_fwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, False, float(eps))
+        both = self.C.qk_rope_fwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, False, float(eps),
+                                  self._reports)
         return both[0], both[1]
 
     def qk_norm_rope_bwd(self, q, k, q_weight, k_weight, rope: AxisRope | None, dq, dk, eps=1e-6, out=None):
@@ -227,7 +229,7 @@ class NativeKernels:
         """
         pos, freqs, pairs, inter = self._rope_args(rope)
         return tuple(self.C.qk_norm_rope_bwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, dq, dk, float(eps),
-                                             [] if out is None else list(out)))
+                                             self._reports, [] if out is None else list(out)))
 
     def packed_plan(self, q_lens, k_lens=None, *, heads, kv_heads, head_dim, causal=False) -> PackedPlan:
         """Work lists of a packed batch, uploaded once; every layer's forward and backward uses them."""

@@ -50,9 +50,11 @@ EXTENSIONS = [
     )
 ]
 # H3_CHECKED_BUILD=1 also builds h3_a100._C_checked: the same kernels with
-# -DH3_BOUNDS_CHECK, where every global access whose index arithmetic is this
-# code's own is checked against its allocation and, if outside, skipped and
-# reported in the status word (tests/test_checked_build.py).
+# -DH3_BOUNDS_CHECK, where the global stores of the GEMM, gather, attention and
+# rotation kernels are checked against their allocations and, if outside,
+# skipped and reported in the status word (tests/test_checked_build.py).  Most loads,
+# TMA accesses (bounded by their tensor maps) and the kernels whose index is a
+# plain i < n (elementwise, the last sum of the norm gradients) are not.
 CHECKED_SOURCES = [
     "csrc/checked/checked_bindings.cpp",
     "csrc/checked/checked_gemm_tcgen05.cu",

@@ -276,3 +276,71 @@ def test_no_rotation_is_a_copy_on_the_gpu(K):  # noqa: F811
     q, k = bf(7, 3, 64), bf(7, 2, 64)
     for got, x in zip(K.rope_axes(q, k, None) + K.rope_axes(q, k, None, inverse=True), (q, k, q, k)):
         assert torch.equal(got, x) and got.data_ptr() != x.data_ptr()
+
+
+# ---------------------------------------------------------------- the bounds-checked build
+@pytest.fixture(scope="module")
+def checked():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    try:
+        from h3_a100 import _C_checked
+    except ImportError:
+        pytest.skip("bounds-checked extension not built (H3_CHECKED_BUILD=1 python setup.py build_ext --inplace)")
+    from h3_a100.ops.native import NativeKernels
+
+    return NativeKernels(torch.device("cuda", 0), wait_limit_s=2.0, extension=_C_checked)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim", [(1, 1, 1, 64), (77, 5, 3, 128), (2371, 14, 2, 64),
+                                                       (9, 43, 42, 128)])
+def test_checked_rotation_and_norms_agree(K, checked, tokens, heads, kv_heads, dim, dtype):  # noqa: F811
+    torch.manual_seed(10)
+    rope = rope_of(tokens, dim, 3, tokens % 2 == 0, "cuda")
+    q, k, qw, kw, dq, dk = norm_inputs(tokens, heads, kv_heads, dim, dtype)
+    results = []
+    for kernels in (K, checked):
+        fused = torch.zeros(tokens, (heads + kv_heads) * dim + 64, dtype=dtype, device="cuda")
+        out = fused[:, 64:64 + heads * dim].view(q.shape), fused[:, 64 + heads * dim:].view(k.shape)
+        results.append(kernels.rope_axes(q, k, rope) + kernels.qk_norm_rope(q, k, qw, kw, rope) +
+                       kernels.qk_norm_rope_bwd(q, k, qw, kw, rope, dq, dk, out=out) + (fused,))
+        kernels.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@gpu
+def test_checked_build_reports_packed_operators(checked, monkeypatch):
+    """With every allocation declared a head short, each kernel reports its last stores and skips them."""
+    torch.manual_seed(11)
+    dim = 128
+    q, k, qw, kw, dq, dk = norm_inputs(33, 5, 3, dim, torch.bfloat16)
+    plan = checked.packed_plan([33], heads=6, kv_heads=3, head_dim=dim, causal=True)
+    split = checked.packed_plan([1], [9000], heads=6, kv_heads=3, head_dim=dim, causal=True)
+    assert split.meta[9] > 0      # joins
+    qa, do, ka, va = bf(33, 6, dim), bf(33, 6, dim), bf(33, 3, dim), bf(33, 3, dim)
+    qs, ks, vs = bf(1, 6, dim), bf(9000, 3, dim), bf(9000, 3, dim)
+    o, lse = checked.attention_packed_fwd(qa, ka, va, plan)
+    grads = [torch.full_like(t, float("nan")) for t in (qa, ka, va)]
+    norm_grads = [torch.full_like(t, float("nan")) for t in (q, k)]
+    checked.check_status()
+
+    def reported(call):
+        monkeypatch.setenv("H3_BOUNDS_SHRINK", str(dim))
+        call()
+        torch.cuda.synchronize()
+        monkeypatch.delenv("H3_BOUNDS_SHRINK")
+        code = int(checked.status[0])
+        checked.status.zero_()
+        return code == 7
+
+    assert reported(lambda: checked.rope_axes(q, None, None))
+    assert reported(lambda: checked.qk_norm_rope(q, k, qw, kw))
+    assert reported(lambda: checked.qk_norm_rope_bwd(q, k, qw, kw, None, dq, dk, out=norm_grads))
+    assert reported(lambda: checked.attention_packed_fwd(qa, ka, va, plan))
+    assert reported(lambda: checked.attention_packed_fwd(qs, ks, vs, split))
+    assert reported(lambda: checked.attention_packed_bwd(qa, ka, va, o, lse, do, plan, out=grads))
+    assert all(torch.isnan(t.view(-1, dim)[-1]).all() for t in grads + norm_grads)
+    # (attention gradients of other rows may lack their delta and lse2, which were declared short too)
+    assert all(not torch.isnan(t.view(-1, dim)[:-1]).any() for t in norm_grads)
