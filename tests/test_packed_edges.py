@@ -7,8 +7,9 @@ import random
 import pytest
 import torch
 
-from h3_a100.ops import AxisRope, TorchKernels
-from test_packed_ops import K, U, bf, norm_turned, rope_of, turned  # noqa: F401  (K is a fixture)
+from h3_a100.ops import AxisRope, PackedPlan, TorchKernels
+from test_packed_ops import (K, U, bf, check_forward, dense, norm_turned, rope_of, turned,  # noqa: F401  (K: a fixture)
+                             within)
 
 _C = pytest.importorskip("h3_a100._C")
 R = TorchKernels()
@@ -344,3 +345,109 @@ def test_checked_build_reports_packed_operators(checked, monkeypatch):
     assert all(torch.isnan(t.view(-1, dim)[-1]).all() for t in grads + norm_grads)
     # (attention gradients of other rows may lack their delta and lse2, which were declared short too)
     assert all(not torch.isnan(t.view(-1, dim)[:-1]).any() for t in norm_grads)
+
+
+# ---------------------------------------------------------------- every form of the attention kernels
+JOINS, FEW, ITEMS, BEGIN, BLOCKS = 9, 19, 5, 6, 7      # places in a plan's meta
+
+
+def forward_items(plan):
+    ints, m = plan.blob.cpu(), plan.meta
+    starts = ints[m[BEGIN]:m[BEGIN] + m[BLOCKS] + 1]
+    return ints[m[ITEMS]:m[ITEMS] + 8 * int(starts[-1])].view(-1, 8).tolist()
+
+
+def form_of(plan):
+    two = any(item[1] > 128 // (plan.heads // plan.kv_heads) for item in forward_items(plan))
+    return plan.meta[JOINS] > 0, bool(plan.meta[FEW]), two
+
+
+# lengths, heads, key heads, and what they ask for: (split key ranges, few rows over many keys, two query tiles an item)
+FORMS = [([70, 200, 1, 130], None, 6, 2, (False, False, False)),
+         ([1031, 200, 777, 1299], None, 8, 8, (False, False, True)),
+         ([130, 9, 300], [9001, 70, 4100], 4, 2, (True, False, False)),
+         ([1290, 9, 300], [9001, 70, 4100], 13, 13, (True, False, True)),
+         ([1, 3, 2], [9001, 257, 6001], 8, 2, (True, True, False))]
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,form", FORMS)
+def test_every_form_keeps_sequences_apart(K, q_lens, k_lens, heads, kv_heads, form, causal, dim):  # noqa: F811
+    """NaN or infinities in one sequence and past the end leave the others' bits alone."""
+    torch.manual_seed(12)
+    plan = K.packed_plan(q_lens, k_lens, heads=heads, kv_heads=kv_heads, head_dim=dim, causal=causal)
+    assert form_of(plan) == form
+    tensors = [bf(plan.q_tokens, heads, dim), bf(plan.k_tokens, kv_heads, dim), bf(plan.k_tokens, kv_heads, dim),
+               bf(plan.q_tokens, heads, dim)]
+
+    def run(q, k, v, do):
+        o, lse = K.attention_packed_fwd(q, k, v, plan)
+        grads = K.attention_packed_bwd(q, k, v, o, lse, do, plan)
+        K.check_status()
+        return (o, lse.t()) + grads
+
+    want = run(*tensors)
+    assert all(torch.isfinite(t).all() for t in want)
+    spans = [slice(n[0], n[0] + n[1]) for n in (plan.q_lens, plan.k_lens)]
+    for bad in (float("nan"), float("inf")):
+        spoilt = []
+        for t, at in zip(tensors, (0, 1, 1, 0)):
+            room = torch.full((t.shape[0] + 300, *t.shape[1:]), bad, dtype=t.dtype, device="cuda")
+            room[:t.shape[0]] = t
+            room[spans[at]] = bad
+            spoilt.append(room[:t.shape[0]])
+        for got, ref, at in zip(run(*spoilt), want, (0, 0, 0, 1, 1)):
+            keep = torch.ones(ref.shape[0], dtype=torch.bool, device="cuda")
+            keep[spans[at]] = False
+            assert torch.equal(got[keep], ref[keep])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,form", FORMS)
+def test_second_query_tiles_see_no_fewer_key_tiles(q_lens, k_lens, heads, kv_heads, form, causal):
+    """The loader fetches an item's keys for its second query tile; the first one's are among them."""
+    lens = list(q_lens), list(q_lens if k_lens is None else k_lens)
+    blob, meta = _C.packed_schedule(*lens, heads, kv_heads, 128, causal, 148)
+    plan = PackedPlan(*lens, heads, kv_heads, 128, causal, blob, tuple(meta))
+    assert form_of(plan) == form
+    bt = 128 // (heads // kv_heads)
+    for _, nq, _, nk, diag, _, _, _ in forward_items(plan):
+        first, second = (-(-min(nk, max(0, n + diag)) // 128) for n in (min(bt, nq), nq))
+        assert 0 < nq <= 2 * bt and first <= second
+
+
+# ---------------------------------------------------------------- a long sequence
+@gpu
+@pytest.mark.parametrize("dim,causal", [(128, False), (128, True), (64, True)])
+def test_attention_of_a_long_sequence(K, dim, causal):  # noqa: F811
+    """The joint sequence of 37,730 tokens beside a short one, two heads on one, in blocks of queries."""
+    torch.manual_seed(13)
+    lens = [37730, 77]
+    plan = K.packed_plan(lens, heads=2, kv_heads=1, head_dim=dim, causal=causal)
+    q, k, v, do = bf(37807, 2, dim), bf(37807, 1, dim), bf(37807, 1, dim), bf(37807, 2, dim)
+    o, lse = K.attention_packed_fwd(q, k, v, plan)
+    grads = K.attention_packed_bwd(q, k, v, o, lse, do, plan)
+    K.check_status()
+    want = {}
+    for at, n, step in ((0, 37730, 1290), (37730, 77, 77)):      # 37,730 is not a multiple of the step
+        ks, vs = k[at:at + n], v[at:at + n]
+        parts = []
+        for i in range(0, n, step):
+            rows = slice(at + i, at + min(i + step, n))
+            part = PackedPlan((rows.stop - rows.start,), (n if not causal else rows.stop - at,), 2, 1, dim, causal)
+            keys = part.k_lens[0]      # under a causal mask the last query of the block sees the last of these
+            parts.append(dense(q[rows], ks[:keys], vs[:keys], part, do=do[rows]))
+        for name in parts[0]:
+            if name in ("dk", "dv", "dk_abs", "dv_abs"):
+                total = torch.zeros(n, 1, dim, dtype=torch.float64, device="cuda")
+                for p in parts:
+                    total[:p[name].shape[0]] += p[name]
+            else:
+                total = torch.cat([p[name] for p in parts], 1 if name in ("lse", "s_abs") else 0)
+            want.setdefault(name, []).append(total)
+    want = {name: torch.cat(t, 1 if name in ("lse", "s_abs") else 0) for name, t in want.items()}
+    check_forward(o, lse, want, dim)
+    for got, name in zip(grads, ("dq", "dk", "dv")):
+        within(got, want[name], want[name + "_abs"] + U * want[name].abs() + 1e-6)
