@@ -17,8 +17,8 @@
 // and no barriers.  The loads of the next batch of heads are issued before the
 // current batch is worked on.
 // Measured (37,730 tokens, 42 + 42 heads of 128, bf16, 1.62 GB): rotation 257 us =
-// 6.3 TB/s, with norms 264 us in a burst and 267 us under the power cap; gradients of
-// 16,411 tokens, 32 + 8 heads (504 MB) 93 us = 5.4 TB/s.
+// 6.3 TB/s, with norms 266 us in a burst and 270 to 275 us under the power cap; gradients of
+// 16,411 tokens, 32 + 8 heads (504 MB) 96 us = 5.2 TB/s.
 // The weight gradients stay in registers over all tokens of a warp (a lane's
 // columns are fixed) and are summed in a fixed order: per block into a partial
 // row, and by a second small kernel over the rows.

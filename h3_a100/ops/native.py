@@ -215,7 +215,7 @@ class NativeKernels:
         return both[0], None if k is None else both[1]
 
     def qk_norm_rope(self, q, k, q_weight, k_weight, rope: AxisRope | None = None, eps=1e-6):
-        """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``), then the rotation."""
+        """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``, of one type), then the rotation."""
         pos, freqs, pairs, inter = self._rope_args(rope)
         both = self.C.qk_rope_fwd(q, k, q_weight, k_weight, pos, freqs, pairs, inter, False, float(eps),
                                   self._reports)
@@ -248,7 +248,7 @@ class NativeKernels:
     def attention_packed_fwd(self, q, k, v, plan: PackedPlan, scale=None):
         """Attention of each sequence of a packed batch with itself -> (o, lse [heads, tokens] fp32).
 
-        bf16, head dim 64 or 128; see ``TorchKernels.attention_packed_fwd``.
+        bf16, head dim 64 or 128, a positive ``scale``; see ``TorchKernels.attention_packed_fwd``.
         """
         blob, meta, scale = self._packed_args(plan, scale)
         o, lse = self.C.attention_packed_fwd(q, k, v, blob, meta, scale, self.status, self.limit_ns)
