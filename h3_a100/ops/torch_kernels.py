@@ -346,7 +346,7 @@ class TorchKernels:
         dtype = torch.promote_types(q.dtype, torch.float32)
         if out is not None and len(out) != 3:
             raise ValueError("out must hold dq, dk and dv")
-        grads = tuple(torch.zeros(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+        grads = tuple(torch.zeros(x.shape, dtype=x.dtype, device=x.device) for x in out or (q, k, v))
         for rq, rk, hidden in self._packed_sequences(plan, q.device):
             if rq.start == rq.stop or rk.start == rk.stop:
                 continue

@@ -185,6 +185,17 @@ def test_torch_gradients_into_inputs():
         R.attention_packed_bwd(q, k, v, o, lse, do, plan, out=(q, k))
 
 
+def test_torch_gradients_keep_the_type_of_out():
+    torch.manual_seed(14)
+    plan = R.packed_plan([6], heads=2, kv_heads=1, head_dim=8)
+    q, k, v, do = (torch.randn(6, h, 8).bfloat16() for h in (2, 1, 1, 2))
+    o, lse = R.attention_packed_fwd(q, k, v, plan)
+    out = tuple(torch.empty(t.shape) for t in (q, k, v))
+    R.attention_packed_bwd(q, k, v, o, lse, do, plan, out=out)
+    short = R.attention_packed_bwd(q, k, v, o, lse, do, plan)
+    assert all(torch.equal(a.bfloat16(), b) and not torch.equal(a, b.float()) for a, b in zip(out, short))
+
+
 @gpu
 def test_gradients_over_inputs_or_each_other_are_refused(K):  # noqa: F811
     plan = K.packed_plan([40, 9], heads=4, kv_heads=2, head_dim=64, causal=True)
